@@ -236,7 +236,7 @@ def exact(case, seed):
         x = s["X"].double()
         scale = x.abs().max(dim=1).values / 127.0
         top = (scale * 127.0).clamp_min(1e-300)
-        # 127 x is exact; a quotient of two 11-bit numbers is never within 2^-13 of a tie without being one
+        # a quotient of 127 times one 11-bit number by another is never within 2^-20 of a tie without being one
         q = torch.round(torch.round(x * 127.0 / top[:, None] * 2.0 ** 20) / 2.0 ** 20)
         return {"values": q * scale[:, None], "scale": scale}
     acc = torch.matmul(s["A"].double(), s["B"].double().mT)
