@@ -285,6 +285,97 @@ pax_status_t pax_ipc_export(const void* device_ptr, pax_ipc_handle_t* out);
 pax_status_t pax_ipc_import(const pax_ipc_handle_t* handle, void** device_ptr);
 pax_status_t pax_ipc_close(void* device_ptr);
 
+/* ---------------------------------------------------------------------------
+ * Feed-forward products (new; no counterpart in the reference).
+ *
+ * The gated feed-forward layer's products next to pax_gemm_ex: the gated
+ * up-projection with its backward pass in fp16, and the 8-bit integer product
+ * that serves quantised weights.  All calls are asynchronous on `stream`,
+ * allocate nothing and keep nothing between calls, so any number of them may
+ * run at once and be captured into graphs.  Zero leading dimensions mean
+ * contiguous.  Dimensions are below 2^31.  Outputs must not overlap inputs or
+ * one another, except where a field says so.  Bases and row pitches that are
+ * multiples of 16 bytes run on the tcgen05 / TMA kernels; any other layout
+ * runs on a slower kernel with the same results.
+ * ------------------------------------------------------------------------- */
+typedef enum {
+    PAX_ACT_SILU      = 0, /* x / (1 + exp(-x))                              */
+    PAX_ACT_GELU_TANH = 1, /* 0.5 x (1 + tanh(sqrt(2/pi)(x + 0.044715 x^3))) */
+    PAX_ACT_GELU_ERF  = 2  /* 0.5 x (1 + erf(x / sqrt 2))                    */
+} pax_activation_t;
+
+/* H = act(X.Wg) * (X.Wu), both products, the activation and the product in
+ * one kernel.  G and U, both or neither, receive the two products X.Wg and
+ * X.Wu, which pax_glu_backward_ex takes.  Sums are fp32; H is rounded to fp16
+ * once, from the unrounded products. */
+typedef struct {
+    const void*      X;  /* fp16 [M][ldx]    tokens                        */
+    const void*      Wg; /* fp16 [D][ldwg]   gate projection               */
+    const void*      Wu; /* fp16 [D][ldwu]   up projection                 */
+    void*            H;  /* fp16 [M][ldh]                                  */
+    void*            G;  /* fp16 [M][ldg], or NULL                         */
+    void*            U;  /* fp16 [M][ldu], or NULL                         */
+    int64_t          M, D, F; /* tokens, model width, feed-forward width   */
+    int64_t          ldx, ldwg, ldwu, ldh, ldg, ldu;
+    pax_activation_t act;
+} pax_glu_desc_t;
+pax_status_t pax_glu_ex(const pax_glu_desc_t* desc, cudaStream_t stream);
+
+/* Gradients of pax_glu_ex from dH and the products G and U it kept:
+ *   dG = dH * U * act'(G),  dU = dH * act(G)          (fp16 [M][F])
+ *   dX = dG.Wg^T + dU.Wu^T                            (fp16 [M][D])
+ *   dWg = X^T.dG,  dWu = X^T.dU                       (dw_dtype [D][F])
+ * dG and dU are written too (they feed the two matrix products, rounded to
+ * fp16) and may be the buffers of G and U themselves.  dX may be NULL, dWg
+ * and dWu may both be NULL; what is NULL is not computed.  accumulate != 0
+ * adds dWg and dWu to what their buffers hold (fp32 only), each element once.
+ * Equal inputs give equal bits from call to call. */
+typedef struct {
+    const void*      dH; /* fp16 [M][lddh]                                 */
+    const void*      X;  /* fp16 [M][ldx]                                  */
+    const void*      Wg; /* fp16 [D][ldwg]                                 */
+    const void*      Wu; /* fp16 [D][ldwu]                                 */
+    const void*      G;  /* fp16 [M][ldg]                                  */
+    const void*      U;  /* fp16 [M][ldu]                                  */
+    void*            dG; /* fp16 [M][lddg]                                 */
+    void*            dU; /* fp16 [M][lddu]                                 */
+    void*            dX; /* fp16 [M][lddx], or NULL                        */
+    void*            dWg; /* dw_dtype [D][lddwg], or NULL                  */
+    void*            dWu; /* dw_dtype [D][lddwu], or NULL                  */
+    int64_t          M, D, F;
+    int64_t          lddh, ldx, ldwg, ldwu, ldg, ldu, lddg, lddu, lddx, lddwg, lddwu;
+    pax_dtype_t      dw_dtype;
+    int              accumulate;
+    pax_activation_t act;
+} pax_glu_grad_desc_t;
+pax_status_t pax_glu_backward_ex(const pax_glu_grad_desc_t* desc, cudaStream_t stream);
+
+/* Rows of fp16 values to int8 codes with one fp32 scale each:
+ *   scale[i] = max_j |X[i][j]| / 127,  Q[i][j] = round(127 X[i][j] / max_j |X[i][j]|)
+ * rounded to nearest, ties to even, of the exact quotient.  Codes lie in
+ * [-127, 127].  A row of zeros has scale 0 and codes 0; a row that holds an
+ * infinity or a NaN has scale NaN and codes 0, so that what is computed from
+ * it is NaN. */
+pax_status_t pax_quantize_rows(const void* X, int64_t ldx, void* Q, int64_t ldq, float* scale, int64_t M, int64_t K,
+                               cudaStream_t stream);
+
+/* C[i][j] = (sum_k A[i][k] B[j][k]) * a_scale[i] * b_scale[j] (+ bias[j]).
+ * A holds tokens and B the weight's output channels, both with K contiguous
+ * (what pax_quantize_rows writes).  The sum is exact in int32: K is at most
+ * 131071, so that no sum of products of codes leaves it. */
+typedef struct {
+    const void*  A;       /* int8 [M][lda]                                 */
+    const void*  B;       /* int8 [N][ldb]                                 */
+    void*        C;       /* c_dtype [M][ldc]                              */
+    const float* a_scale; /* fp32 [M], one per token                       */
+    const float* b_scale; /* fp32 [N], one per output channel              */
+    const void*  bias;    /* fp16 [N], or NULL                             */
+    int64_t      M, N, K;
+    int64_t      lda, ldb, ldc;
+    pax_dtype_t  c_dtype;
+} pax_gemm_i8_desc_t;
+pax_status_t pax_gemm_i8_ex(const pax_gemm_i8_desc_t* desc, cudaStream_t stream);
+
 /* The algorithm pax_gemm_ex would run for desc with algo = PAX_ALGO_AUTO (new;
  * host-only, launches nothing). */
 pax_algo_t pax_gemm_select_algo(const pax_gemm_desc_t* desc);
@@ -439,6 +530,9 @@ const char*  pax_version(void);
  * library, so that bindings can check their struct layouts. */
 size_t       pax_sizeof_buffer(void);
 size_t       pax_sizeof_gemm_desc(void);
+/* The same for the feed-forward descriptors: which = 0 pax_glu_desc_t,
+ * 1 pax_glu_grad_desc_t, 2 pax_gemm_i8_desc_t (0 for any other number). */
+size_t       pax_sizeof_feed_forward_desc(int which);
 
 #ifdef __cplusplus
 } /* extern "C" */

@@ -51,6 +51,27 @@ class GemmDesc(ctypes.Structure):
     ]
 
 
+class GluDesc(ctypes.Structure):
+    """pax_glu_desc_t (include/pax.h)."""
+    _fields_ = ([(n, ctypes.c_void_p) for n in ("X", "Wg", "Wu", "H", "G", "U")]
+                + [(n, ctypes.c_int64) for n in ("M", "D", "F", "ldx", "ldwg", "ldwu", "ldh", "ldg", "ldu")]
+                + [("act", ctypes.c_int)])
+
+
+class GluGradDesc(ctypes.Structure):
+    """pax_glu_grad_desc_t (include/pax.h)."""
+    _fields_ = ([(n, ctypes.c_void_p) for n in ("dH", "X", "Wg", "Wu", "G", "U", "dG", "dU", "dX", "dWg", "dWu")]
+                + [(n, ctypes.c_int64) for n in ("M", "D", "F", "lddh", "ldx", "ldwg", "ldwu", "ldg", "ldu", "lddg", "lddu",
+                                                 "lddx", "lddwg", "lddwu")]
+                + [(n, ctypes.c_int) for n in ("dw_dtype", "accumulate", "act")])
+
+
+class GemmI8Desc(ctypes.Structure):
+    """pax_gemm_i8_desc_t (include/pax.h)."""
+    _fields_ = ([(n, ctypes.c_void_p) for n in ("A", "B", "C", "a_scale", "b_scale", "bias")]
+                + [(n, ctypes.c_int64) for n in ("M", "N", "K", "lda", "ldb", "ldc")] + [("c_dtype", ctypes.c_int)])
+
+
 class IpcHandle(ctypes.Structure):
     """pax_ipc_handle_t (include/pax.h)."""
     _fields_ = [("handle", ctypes.c_ubyte * 64), ("offset", ctypes.c_uint64)]
@@ -107,6 +128,12 @@ def _declare(L: ctypes.CDLL) -> None:
         "pax_gemm_pipeline_stages": ([ctypes.POINTER(GemmDesc)], i),
         "pax_gemm_smem_bytes": ([ctypes.POINTER(GemmDesc)], sz),
         "pax_gemm_skinny_noalloc": ([ctypes.POINTER(GemmDesc), P], i),
+        # feed-forward products
+        "pax_glu_ex": ([ctypes.POINTER(GluDesc), P], i),
+        "pax_glu_backward_ex": ([ctypes.POINTER(GluGradDesc), P], i),
+        "pax_quantize_rows": ([P, ctypes.c_int64, P, ctypes.c_int64, P, ctypes.c_int64, ctypes.c_int64, P], i),
+        "pax_gemm_i8_ex": ([ctypes.POINTER(GemmI8Desc), P], i),
+        "pax_sizeof_feed_forward_desc": ([i], sz),
         # Lean-extraction names (64-bit sizes, pointers as integers)
         "pax_gemm_wmma_verified": ([u64] * 6, None),
         "pax_gemm_ptx_verified": ([u64] * 6, None),
@@ -181,5 +208,7 @@ def load() -> ctypes.CDLL:
         raise ImportError("pax_buffer_t layout mismatch between libpax_b200.so and the Python binding")
     if L.pax_sizeof_gemm_desc() != ctypes.sizeof(GemmDesc):
         raise ImportError("pax_gemm_desc_t layout mismatch between libpax_b200.so and the Python binding")
+    for which, desc in enumerate((GluDesc, GluGradDesc, GemmI8Desc)):
+        if L.pax_sizeof_feed_forward_desc(which) != ctypes.sizeof(desc):
+            raise ImportError(f"{desc.__name__} layout mismatch between libpax_b200.so and the Python binding")
     return L
-

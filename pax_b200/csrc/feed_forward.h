@@ -1,0 +1,51 @@
+// feed_forward.h -- host-side interface of the feed-forward products: the
+// validated problems that feed_forward.cpp hands to the kernel translation
+// units.  Not part of the public ABI.
+#pragma once
+
+#include "internal.h"
+
+namespace pax {
+
+// H = act(X.Wg) * (X.Wu); G and U may be null.
+struct GluProblem {
+    const __half *X, *Wg, *Wu;
+    __half *H, *G, *U;
+    long long M, D, F;
+    long long ldx, ldwg, ldwu, ldh, ldg, ldu;
+    int act;
+};
+
+struct GluGradProblem {
+    const __half *dH, *X, *Wg, *Wu, *G, *U;
+    __half *dG, *dU, *dX;  // dX may be null
+    void *dWg, *dWu;       // may be null
+    long long M, D, F;
+    long long lddh, ldx, ldwg, ldwu, ldg, ldu, lddg, lddu, lddx, lddwg, lddwu;
+    bool dw_f16, accumulate;
+    int act;
+};
+
+struct I8Problem {
+    const int8_t *A, *B;
+    void* C;
+    const float *a_scale, *b_scale;
+    const __half* bias;  // may be null
+    long long M, N, K;
+    long long lda, ldb, ldc;
+    bool c_f16;
+};
+
+// feed_forward_any.cu: any layout, any alignment, empty sums.
+pax_status_t glu_any(const GluProblem& p, cudaStream_t stream);
+pax_status_t glu_dx_any(const GluGradProblem& p, cudaStream_t stream);
+pax_status_t glu_dw_any(const GluGradProblem& p, cudaStream_t stream);
+pax_status_t gemm_i8_any(const I8Problem& p, cudaStream_t stream);
+
+// feed_forward_rows.cu: the elementwise part of the backward pass, and the
+// quantisation of rows.
+pax_status_t glu_grad_rows(const GluGradProblem& p, cudaStream_t stream);
+pax_status_t quantize_rows(const __half* X, long long ldx, int8_t* Q, long long ldq, float* scale, long long M,
+                           long long K, cudaStream_t stream);
+
+}  // namespace pax
