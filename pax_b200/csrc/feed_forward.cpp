@@ -167,7 +167,7 @@ pax_status_t pax_glu_ex(const pax_glu_desc_t* desc, cudaStream_t stream) {
     if (st != PAX_OK) return st;
     if (p.M == 0 || p.F == 0) return report_status(PAX_OK, "");
     if ((st = device_ok("pax_glu_ex")) != PAX_OK) return st;
-    return done(glu_any(p, stream), "pax_glu_ex");
+    return done(glu_tc_ok(p) ? glu_tc(p, stream) : glu_any(p, stream), "pax_glu_ex");
 }
 
 pax_status_t pax_glu_backward_ex(const pax_glu_grad_desc_t* desc, cudaStream_t stream) {
@@ -177,8 +177,14 @@ pax_status_t pax_glu_backward_ex(const pax_glu_grad_desc_t* desc, cudaStream_t s
     if (p.M == 0 && (p.D == 0 || p.F == 0 || !p.dWg)) return report_status(PAX_OK, "");
     if ((st = device_ok("pax_glu_backward_ex")) != PAX_OK) return st;
     st = glu_grad_rows(p, stream);
-    if (st == PAX_OK && p.dX) st = glu_dx_any(p, stream);
-    if (st == PAX_OK && p.dWg) st = glu_dw_any(p, stream);
+    if (st == PAX_OK && (p.dX || p.dWg)) {
+        if (glu_back_tc_ok(p)) {
+            st = glu_back_tc(p, stream);
+        } else {
+            if (p.dX) st = glu_dx_any(p, stream);
+            if (st == PAX_OK && p.dWg) st = glu_dw_any(p, stream);
+        }
+    }
     return done(st, "pax_glu_backward_ex");
 }
 
@@ -204,7 +210,7 @@ pax_status_t pax_gemm_i8_ex(const pax_gemm_i8_desc_t* desc, cudaStream_t stream)
     if (st != PAX_OK) return st;
     if (p.M == 0 || p.N == 0) return report_status(PAX_OK, "");
     if ((st = device_ok("pax_gemm_i8_ex")) != PAX_OK) return st;
-    return done(gemm_i8_any(p, stream), "pax_gemm_i8_ex");
+    return done(gemm_i8_tc_ok(p) ? gemm_i8_tc(p, stream) : gemm_i8_any(p, stream), "pax_gemm_i8_ex");
 }
 
 size_t pax_sizeof_feed_forward_desc(int which) {

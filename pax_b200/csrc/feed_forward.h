@@ -42,6 +42,17 @@ pax_status_t glu_dx_any(const GluGradProblem& p, cudaStream_t stream);
 pax_status_t glu_dw_any(const GluGradProblem& p, cudaStream_t stream);
 pax_status_t gemm_i8_any(const I8Problem& p, cudaStream_t stream);
 
+// feed_forward_tc.cu: tcgen05 kernels; *_ok says whether the problem's
+// layout lets them.  glu_back_tc takes dG and dU as glu_grad_rows left them.
+bool glu_tc_ok(const GluProblem& p);
+pax_status_t glu_tc(const GluProblem& p, cudaStream_t stream);
+bool glu_back_tc_ok(const GluGradProblem& p);
+pax_status_t glu_back_tc(const GluGradProblem& p, cudaStream_t stream);
+bool gemm_i8_tc_ok(const I8Problem& p);
+pax_status_t gemm_i8_tc(const I8Problem& p, cudaStream_t stream);
+int read_clear_device_error_ff_tc();
+bool set_wait_limit_ff_tc(unsigned long long ns);
+
 // feed_forward_rows.cu: the elementwise part of the backward pass, and the
 // quantisation of rows.
 pax_status_t glu_grad_rows(const GluGradProblem& p, cudaStream_t stream);

@@ -1,0 +1,180 @@
+// feed_forward_tc.cu -- launches of the tcgen05 feed-forward kernel
+// (feed_forward_tc.cuh).
+#include "feed_forward_tc.cuh"
+
+namespace pax {
+
+namespace {
+
+constexpr CUtensorMapDataType kF16 = CU_TENSOR_MAP_DATA_TYPE_FLOAT16, kF32 = CU_TENSOR_MAP_DATA_TYPE_FLOAT32,
+                              kU8 = CU_TENSOR_MAP_DATA_TYPE_UINT8;
+
+bool rows16(const void* p, long long ld, int elem) {
+    return (reinterpret_cast<uintptr_t>(p) & 15u) == 0 && (ld * elem) % 16 == 0;
+}
+
+// Output rows that TMA stores may write: a store covers whole 16-byte units,
+// so that a width that ends inside one would write beyond it.
+bool out16(const void* p, long long cols, long long ld, int elem) {
+    return rows16(p, ld, elem) && (cols * elem) % 16 == 0;
+}
+
+int up(long long a, int b) { return (int)((a + b - 1) / b); }
+
+// Tiles run in column-major groups of this many tile rows (as in
+// gemm_tc.cuh, where 16 measured best at every shape).
+constexpr int kGroupM = 16;
+
+template <int ACT>
+pax_status_t launch_glu(const FfMaps& maps, const FfParams& p, cudaStream_t stream) {
+    const int most = ff_units<FF_GLU, ACT, __half>(current_device());
+    if (most <= 0) return PAX_ERR_CUDA;
+    const long long tiles = (long long)p.tiles_m * p.tiles_n;
+    return ff_launch<FF_GLU, ACT, __half>(maps, p, (int)(tiles < most ? tiles : most), stream);
+}
+
+template <typename OutT>
+pax_status_t launch_back(const FfMaps& maps, FfParams& p, cudaStream_t stream) {
+    const int most = ff_units<FF_BACK, 0, OutT>(current_device());
+    if (most <= 0) return PAX_ERR_CUDA;
+    const long long items = (long long)p.nx + p.nw;
+    const int units = (int)(items < most ? items : most);
+    p.x_rem = p.nx % units;
+    p.w_extra = 0;
+    if (p.x_rem > 0 && p.nw > 0) p.w_extra = (p.kbs + p.kbs_w / 2) / p.kbs_w;
+    return ff_launch<FF_BACK, 0, OutT>(maps, p, units, stream);
+}
+
+template <typename OutT>
+pax_status_t launch_i8(const FfMaps& maps, const FfParams& p, cudaStream_t stream) {
+    const int most = ff_units<FF_I8, 0, OutT>(current_device());
+    if (most <= 0) return PAX_ERR_CUDA;
+    const long long tiles = (long long)p.tiles_m * p.tiles_n;
+    return ff_launch<FF_I8, 0, OutT>(maps, p, (int)(tiles < most ? tiles : most), stream);
+}
+
+bool tiles_ok(long long a, long long b) { return a * b <= 0x3fffffffLL; }
+
+}  // namespace
+
+bool glu_tc_ok(const GluProblem& q) {
+    return q.D > 0 && rows16(q.X, q.ldx, 2) && rows16(q.Wg, q.ldwg, 2) && rows16(q.Wu, q.ldwu, 2) &&
+           out16(q.H, q.F, q.ldh, 2) && (!q.G || (out16(q.G, q.F, q.ldg, 2) && out16(q.U, q.F, q.ldu, 2))) &&
+           tiles_ok(up(q.M, 256), up(q.F, 128));
+}
+
+pax_status_t glu_tc(const GluProblem& q, cudaStream_t stream) {
+    FfMaps maps;
+    FfParams p = {};
+    CUtensorMap* m = maps.m;
+    bool ok = ff_map(&m[MG_X], q.X, kF16, 2, q.M, q.D, q.ldx, 64, 128) &&
+              ff_map(&m[MG_WG], q.Wg, kF16, 2, q.D, q.F, q.ldwg, 64, 64) &&
+              ff_map(&m[MG_WU], q.Wu, kF16, 2, q.D, q.F, q.ldwu, 64, 64) &&
+              ff_map(&m[MG_H], q.H, kF16, 2, q.M, q.F, q.ldh, 64, 32);
+    if (ok && q.G)
+        ok = ff_map(&m[MG_G], q.G, kF16, 2, q.M, q.F, q.ldg, 64, 32) &&
+             ff_map(&m[MG_U], q.U, kF16, 2, q.M, q.F, q.ldu, 64, 32);
+    if (!ok) return PAX_ERR_CUDA;
+    for (int i = q.G ? MG_U + 1 : MG_H + 1; i < 10; ++i) m[i] = m[MG_X];
+    p.M = (int)q.M;
+    p.N = (int)q.F;
+    p.tiles_m = up(q.M, 256);
+    p.tiles_n = up(q.F, 128);
+    p.kbs = up(q.D, 64);
+    p.group_m = kGroupM;
+    p.save = q.G != nullptr;
+    if (q.act == ACT_SILU) return launch_glu<ACT_SILU>(maps, p, stream);
+    if (q.act == ACT_GELU_TANH) return launch_glu<ACT_GELU_TANH>(maps, p, stream);
+    return launch_glu<ACT_GELU_ERF>(maps, p, stream);
+}
+
+bool glu_back_tc_ok(const GluGradProblem& q) {
+    const int w = q.dw_f16 ? 2 : 4;
+    return q.M > 0 && q.D > 0 && q.F > 0 && rows16(q.dG, q.lddg, 2) && rows16(q.dU, q.lddu, 2) &&
+           (!q.dX || (rows16(q.Wg, q.ldwg, 2) && rows16(q.Wu, q.ldwu, 2) && out16(q.dX, q.D, q.lddx, 2))) &&
+           (!q.dWg || (rows16(q.X, q.ldx, 2) && out16(q.dWg, q.F, q.lddwg, w) && out16(q.dWu, q.F, q.lddwu, w))) &&
+           tiles_ok(up(q.M, 256), up(q.D, 256)) && tiles_ok(up(q.D, 256), 2LL * up(q.F, 256));
+}
+
+pax_status_t glu_back_tc(const GluGradProblem& q, cudaStream_t stream) {
+    FfMaps maps;
+    FfParams p = {};
+    CUtensorMap* m = maps.m;
+    const CUtensorMapDataType wt = q.dw_f16 ? kF16 : kF32;
+    const int we = q.dw_f16 ? 2 : 4;
+    bool ok = ff_map(&m[MB_DGK], q.dG, kF16, 2, q.M, q.F, q.lddg, 64, 128) &&
+              ff_map(&m[MB_DUK], q.dU, kF16, 2, q.M, q.F, q.lddu, 64, 128) &&
+              ff_map(&m[MB_DGN], q.dG, kF16, 2, q.M, q.F, q.lddg, 64, 64) &&
+              ff_map(&m[MB_DUN], q.dU, kF16, 2, q.M, q.F, q.lddu, 64, 64);
+    m[MB_WGK] = m[MB_WUK] = m[MB_DX] = m[MB_XN] = m[MB_DWG] = m[MB_DWU] = m[MB_DGK];
+    if (ok && q.dX)
+        ok = ff_map(&m[MB_WGK], q.Wg, kF16, 2, q.D, q.F, q.ldwg, 64, 128) &&
+             ff_map(&m[MB_WUK], q.Wu, kF16, 2, q.D, q.F, q.ldwu, 64, 128) &&
+             ff_map(&m[MB_DX], q.dX, kF16, 2, q.M, q.D, q.lddx, 64, 32);
+    if (ok && q.dWg)
+        ok = ff_map(&m[MB_XN], q.X, kF16, 2, q.M, q.D, q.ldx, 64, 64) &&
+             ff_map(&m[MB_DWG], q.dWg, wt, we, q.D, q.F, q.lddwg, 128 / we, 32) &&
+             ff_map(&m[MB_DWU], q.dWu, wt, we, q.D, q.F, q.lddwu, 128 / we, 32);
+    if (!ok) return PAX_ERR_CUDA;
+    p.M = (int)q.M;
+    p.D = (int)q.D;
+    p.F = (int)q.F;
+    p.N = p.D;
+    p.tiles_m = up(q.M, 256);
+    p.tiles_n = up(q.D, 256);
+    p.half_kbs = up(q.F, 64);
+    p.kbs = 2 * p.half_kbs;
+    p.group_m = kGroupM;
+    p.wt_m = up(q.D, 256);
+    p.wt_n = up(q.F, 256);
+    p.kbs_w = up(q.M, 64);
+    p.nx = q.dX ? p.tiles_m * p.tiles_n : 0;
+    p.nw = q.dWg ? p.wt_m * 2 * p.wt_n : 0;
+    p.accumulate = q.accumulate;
+    return q.dw_f16 ? launch_back<__half>(maps, p, stream) : launch_back<float>(maps, p, stream);
+}
+
+bool gemm_i8_tc_ok(const I8Problem& q) {
+    return q.K > 0 && rows16(q.A, q.lda, 1) && rows16(q.B, q.ldb, 1) && tiles_ok(up(q.M, 256), up(q.N, 256));
+}
+
+pax_status_t gemm_i8_tc(const I8Problem& q, cudaStream_t stream) {
+    FfMaps maps;
+    FfParams p = {};
+    CUtensorMap* m = maps.m;
+    const int ce = q.c_f16 ? 2 : 4;
+    bool ok = ff_map(&m[MI_A], q.A, kU8, 1, q.M, q.K, q.lda, 128, 128) &&
+              ff_map(&m[MI_B], q.B, kU8, 1, q.N, q.K, q.ldb, 128, 128);
+    p.c_tma = out16(q.C, q.N, q.ldc, ce);
+    m[MI_C] = m[MI_A];
+    if (ok && p.c_tma) ok = ff_map(&m[MI_C], q.C, q.c_f16 ? kF16 : kF32, ce, q.M, q.N, q.ldc, 128 / ce, 32);
+    if (!ok) return PAX_ERR_CUDA;
+    for (int i = MI_C + 1; i < 10; ++i) m[i] = m[MI_A];
+    p.M = (int)q.M;
+    p.N = (int)q.N;
+    p.tiles_m = up(q.M, 256);
+    p.tiles_n = up(q.N, 256);
+    p.kbs = up(q.K, 128);
+    p.group_m = kGroupM;
+    p.C = q.C;
+    p.ldc = q.ldc;
+    p.sa = q.a_scale;
+    p.sb = q.b_scale;
+    p.bias = q.bias;
+    p.sb_vec = (reinterpret_cast<uintptr_t>(q.b_scale) & 15u) == 0;
+    p.bias_vec = (reinterpret_cast<uintptr_t>(q.bias) & 15u) == 0;
+    return q.c_f16 ? launch_i8<__half>(maps, p, stream) : launch_i8<float>(maps, p, stream);
+}
+
+int read_clear_device_error_ff_tc() {
+    int v = 0, z = 0;
+    if (cudaMemcpyFromSymbol(&v, g_pax_device_error, sizeof(int)) != cudaSuccess) return -1;
+    if (v) cudaMemcpyToSymbol(g_pax_device_error, &z, sizeof(int));
+    return v;
+}
+
+bool set_wait_limit_ff_tc(unsigned long long ns) {
+    return cudaMemcpyToSymbol(g_pax_wait_limit_ns, &ns, sizeof(ns)) == cudaSuccess;
+}
+
+}  // namespace pax

@@ -40,8 +40,8 @@
 #include "internal.h"
 #include "sm100.cuh"
 #include "epilogue.cuh"
+#include "tmap.h"
 
-#include <cudaTypedefs.h>
 #include <stdlib.h>
 #include <string.h>
 #include <mutex>
@@ -734,20 +734,6 @@ __global__ void __launch_bounds__(64 + 32 * 8, 1)
 // ======================================================================
 // Host side
 // ======================================================================
-
-static PFN_cuTensorMapEncodeTiled_v12000 tensor_map_encoder() {
-    static PFN_cuTensorMapEncodeTiled_v12000 fn = nullptr;
-    static std::once_flag once;
-    std::call_once(once, [] {
-        void* p = nullptr;
-        cudaDriverEntryPointQueryResult q;
-        if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &p, 12000, cudaEnableDefault, &q) ==
-                cudaSuccess &&
-            q == cudaDriverEntryPointSuccess)
-            fn = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(p);
-    });
-    return fn;
-}
 
 // 3-D tensor map of `depth` row-major matrices: `inner` contiguous elements
 // per row, `outer` rows `pitch` bytes apart, matrices `zstride` bytes apart;

@@ -89,6 +89,23 @@ def test_glu_strided_operands_and_outputs(gen, M):
         assert (b[:, F:] == 7).all() and (b[0] == 7).all() and (b[-1] == 7).all()
 
 
+@pytest.mark.parametrize("M", [3, 150])
+def test_sums_that_end_inside_a_16_byte_unit(gen, M):
+    """Aligned row pitches with odd lengths: what follows a row's end is NaN or a code, and must not be read into the sum."""
+    for D, F in ((133, 264), (70, 137)):
+        X, (Wg, Wu) = padded(randn(gen, M, D), 200 - D), (padded(w, 280 - F) for w in weights(gen, D, F))
+        buf = torch.full((M, 280), 7.0, device=gen.device, dtype=F16)
+        close(pax_b200.glu(X, Wg, Wu, out=buf[:, :F]), glu(X, Wg, Wu, "silu")["H"], "H")
+        assert (buf[:, F:] == 7).all()
+        a = [padded(t, 280 - t.shape[1]) for t in back_inputs(gen, M, D, F)]
+        ref = glu_grad(*a, "silu")
+        for got, what in zip(pax_b200.glu_backward(*a), ("dX", "dWg", "dWu")):
+            close(got, ref[what], what)
+    A, B = padded(codes(gen, M, 137), 160 - 137, 55), padded(codes(gen, 40, 137), 176 - 137, 55)
+    sa, sb = torch.rand(M, generator=gen, device=gen.device) * 1e-2, torch.rand(40, generator=gen, device=gen.device) * 1e-2
+    close(pax_b200.gemm_i8(A, B, sa, sb), gemm_i8(A, B, sa, sb, None, True), "C")
+
+
 @pytest.mark.parametrize("M", [2, 100])
 def test_glu_unaligned_bases(gen, M):
     D, F = 64, 128
