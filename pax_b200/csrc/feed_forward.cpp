@@ -167,7 +167,8 @@ pax_status_t pax_glu_ex(const pax_glu_desc_t* desc, cudaStream_t stream) {
     if (st != PAX_OK) return st;
     if (p.M == 0 || p.F == 0) return report_status(PAX_OK, "");
     if ((st = device_ok("pax_glu_ex")) != PAX_OK) return st;
-    return done(glu_tc_ok(p) ? glu_tc(p, stream) : glu_any(p, stream), "pax_glu_ex");
+    st = glu_skinny_ok(p) ? glu_skinny(p, stream) : glu_tc_ok(p) ? glu_tc(p, stream) : glu_any(p, stream);
+    return done(st, "pax_glu_ex");
 }
 
 pax_status_t pax_glu_backward_ex(const pax_glu_grad_desc_t* desc, cudaStream_t stream) {
@@ -210,7 +211,10 @@ pax_status_t pax_gemm_i8_ex(const pax_gemm_i8_desc_t* desc, cudaStream_t stream)
     if (st != PAX_OK) return st;
     if (p.M == 0 || p.N == 0) return report_status(PAX_OK, "");
     if ((st = device_ok("pax_gemm_i8_ex")) != PAX_OK) return st;
-    return done(gemm_i8_tc_ok(p) ? gemm_i8_tc(p, stream) : gemm_i8_any(p, stream), "pax_gemm_i8_ex");
+    st = gemm_i8_skinny_ok(p) ? gemm_i8_skinny(p, stream)
+         : gemm_i8_tc_ok(p)   ? gemm_i8_tc(p, stream)
+                              : gemm_i8_any(p, stream);
+    return done(st, "pax_gemm_i8_ex");
 }
 
 size_t pax_sizeof_feed_forward_desc(int which) {

@@ -53,6 +53,14 @@ pax_status_t gemm_i8_tc(const I8Problem& p, cudaStream_t stream);
 int read_clear_device_error_ff_tc();
 bool set_wait_limit_ff_tc(unsigned long long ns);
 
+// feed_forward_skinny.cu: at most 64 tokens.
+bool glu_skinny_ok(const GluProblem& p);
+pax_status_t glu_skinny(const GluProblem& p, cudaStream_t stream);
+bool gemm_i8_skinny_ok(const I8Problem& p);
+pax_status_t gemm_i8_skinny(const I8Problem& p, cudaStream_t stream);
+int read_clear_device_error_ff_skinny();
+bool set_wait_limit_ff_skinny(unsigned long long ns);
+
 // feed_forward_rows.cu: the elementwise part of the backward pass, and the
 // quantisation of rows.
 pax_status_t glu_grad_rows(const GluGradProblem& p, cudaStream_t stream);
