@@ -8,16 +8,18 @@
 //   gated   64 columns of Wg and the same 64 of Wu (MN-major, as they lie)
 //   8-bit   128 rows of B (K-major, as they lie)
 //
-// One tile of weight columns is too little work to go round 148 SMs, so a
+// A tile of weight columns is too coarse a unit of work for 148 SMs, so a
 // cluster of S CTAs shares each tile along K: CTA r takes k-blocks r, r + S,
 // and so on, which streams neighbouring rows at the same time.  The partial
 // sums meet in distributed shared memory: CTA j owns the j-th part of the
 // tile's columns, every CTA stores its partial sums of that part straight
-// into CTA j's buffer, and CTA j adds the S contributions in CTA order,
-// applies the epilogue and stores.  No global workspace, no atomics, and the
-// same bits every time.  Clusters are persistent; the ring keeps loading the
-// next tile's weights while the last one is reduced.  S is the one of 1..8
-// that leaves the busiest cluster with the fewest k-blocks.
+// into CTA j's (by then idle) ring, and CTA j adds the S contributions in CTA
+// order, applies the epilogue and stores.  No global workspace, no atomics,
+// and the same bits every time.
+//
+// A cluster computes one tile and ends.  Two CTAs are resident per SM, so
+// that one streams while the other starts up or reduces, and the hardware
+// hands the next cluster to whichever SMs are free.
 //
 // 192 threads: warp 0 TMA producer, warp 1 MMA issuer, warps 2-5 epilogue
 // (one TMEM lane, i.e. one weight column, per thread).  Every wait is bounded
@@ -33,8 +35,7 @@ namespace {
 enum : int { FS_GLU = 0, FS_I8 = 1 };
 
 struct FsParams {
-    int M, N, tiles, kbs;  // tokens, weight columns, column tiles, k-blocks
-    int clusters;
+    int M, N, kbs;  // tokens, weight columns, k-blocks
     // FS_GLU
     __half *H, *G, *U;
     long long ldh, ldg, ldu;
@@ -49,20 +50,19 @@ struct FsParams {
 
 template <int MODE, int MP>
 struct FsCfg {
-    static constexpr int KB = MODE == FS_I8 ? 256 : 128;   // k of a ring slot: two 128-byte rows
+    static constexpr int KB = MODE == FS_I8 ? 128 : 64;    // k of a ring slot: 128 bytes
     static constexpr int TILE = MODE == FS_I8 ? 128 : 64;  // output columns of a tile
-    static constexpr uint32_t W_BYTES = 2 * 16384, X_BYTES = 2 * MP * 128, STAGE_BYTES = W_BYTES + X_BYTES;
-    static constexpr int RB = MP <= 32 ? 2 : 1;            // receive buffers
-    // A buffer holds S parts of at most ceil(TILE / S) columns (two values
-    // each for the gated product) for MP tokens: up to 128 + 2 (S - 1) values
-    // a token.
-    static constexpr uint32_t RECV_FLOATS = MP * 144;
-    static constexpr uint32_t FIXED = 1024 + RB * RECV_FLOATS * 4 + 256;
-    static constexpr int STAGES = (int)((232448 - FIXED) / STAGE_BYTES) > 6 ? 6 : (int)((232448 - FIXED) / STAGE_BYTES);
-    static constexpr uint32_t NUM_BARS = 2 * STAGES + 4 + 2 * RB + 1;
-    static constexpr size_t SMEM_BYTES = 1024 + (size_t)STAGES * STAGE_BYTES + RB * RECV_FLOATS * 4 + NUM_BARS * 8 + 16;
-    static constexpr uint32_t TMEM_COLS = 2 * MP <= 32 ? 32 : 2 * MP <= 64 ? 64 : 128;
-    static_assert(SMEM_BYTES <= 232448 && STAGES >= 3, "shared memory budget");
+    static constexpr uint32_t W_BYTES = 16384, X_BYTES = MP * 128, STAGE_BYTES = W_BYTES + X_BYTES;
+    // As many slots as let two CTAs share an SM.
+    static constexpr int STAGES = (int)((113 * 1024 - 1024 - 256) / STAGE_BYTES);
+    static constexpr uint32_t NUM_BARS = 2 * STAGES + 1;
+    static constexpr size_t SMEM_BYTES = 1024 + (size_t)STAGES * STAGE_BYTES + NUM_BARS * 8 + 16;
+    static constexpr uint32_t TMEM_COLS = MP <= 32 ? 32 : 64;
+    // The reduction's buffer in the ring: S parts of at most ceil(TILE / S)
+    // columns (two values each for the gated product) for MP tokens, up to
+    // 128 + 2 (S - 1) values a token.
+    static_assert(MP * 144 * 4 <= STAGES * STAGE_BYTES, "the ring holds the contributions");
+    static_assert(SMEM_BYTES <= 113 * 1024 && STAGES >= 4, "shared memory of half an SM");
 };
 
 // First column of part j of a tile shared by S CTAs.
@@ -71,101 +71,77 @@ __device__ __forceinline__ int part_start(int j, int S) {
     return (j * TILE + S - 1) / S;
 }
 
-__device__ __forceinline__ void epilogue_sync() { asm volatile("bar.sync 1, 128;" ::: "memory"); }
-
 template <int MODE, int MP>
-__global__ void __launch_bounds__(192, 1)
+__global__ void __launch_bounds__(192, 2)
     ff_skinny_kernel(const __grid_constant__ CUtensorMap tmW0, const __grid_constant__ CUtensorMap tmW1,
                      const __grid_constant__ CUtensorMap tmX, const __grid_constant__ FsParams p) {
     using Cfg = FsCfg<MODE, MP>;
-    constexpr int STAGES = Cfg::STAGES, RB = Cfg::RB, TILE = Cfg::TILE;
+    constexpr int STAGES = Cfg::STAGES, TILE = Cfg::TILE;
     extern __shared__ __align__(1024) uint8_t smem_raw[];
     uint8_t* smem =
         reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-    float* recv = reinterpret_cast<float*>(smem + STAGES * Cfg::STAGE_BYTES);
-    uint64_t* bars = reinterpret_cast<uint64_t*>(recv + RB * Cfg::RECV_FLOATS);
+    uint64_t* bars = reinterpret_cast<uint64_t*>(smem + STAGES * Cfg::STAGE_BYTES);
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + Cfg::NUM_BARS);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
     const uint32_t full0 = smem_u32(bars);
     const uint32_t empty0 = full0 + 8u * STAGES;
-    const uint32_t tfull0 = empty0 + 8u * STAGES;
-    const uint32_t tempty0 = tfull0 + 16u;
-    const uint32_t recv0 = tempty0 + 16u;       // [RB]: the S contributions are in
-    const uint32_t credit0 = recv0 + 8u * RB;   // [RB]: all owners have read what this CTA sent
-    const uint32_t drain_bar = credit0 + 8u * RB;
+    const uint32_t done_bar = empty0 + 8u * STAGES;  // every MMA has finished
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     int S;
     asm("mov.u32 %0, %%cluster_nctarank;" : "=r"(S));
     const int rank = (int)cluster_ctarank();
-    const int first = (int)blockIdx.x / S;  // this cluster's tiles: first, first + clusters, ...
+    const int tile = (int)blockIdx.x / S;
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < STAGES; ++s) {
             mbar_init(full0 + 8u * s, 1);
             mbar_init(empty0 + 8u * s, 1);
         }
-        for (int b = 0; b < 2; ++b) {
-            mbar_init(tfull0 + 8u * b, 1);
-            mbar_init(tempty0 + 8u * b, 4);
-        }
-        for (int b = 0; b < RB; ++b) {
-            mbar_init(recv0 + 8u * b, 4 * S);
-            mbar_init(credit0 + 8u * b, S);
-        }
-        mbar_init(drain_bar, 1);
+        mbar_init(done_bar, 1);
         *abort_flag = 0;
         fence_mbar_init();
-        tma_prefetch_desc(&tmW0);
-        tma_prefetch_desc(&tmX);
-        if (MODE == FS_GLU) tma_prefetch_desc(&tmW1);
     }
     if (warp == 1) {
         tmem_alloc<1>(smem_u32(tmem_slot), Cfg::TMEM_COLS);
         tmem_relinquish<1>();
     }
     tc_fence_before();
-    cluster_sync();  // barriers initialised before a peer's first arrival
+    __syncthreads();
     tc_fence_after();
     const uint32_t tmem_base = *tmem_slot;
     if (threadIdx.x == 0) pdl_launch_dependents();
 
+    float v[MP];
+    const int q = warp & 3;  // TMEM lane quarter an epilogue warp may read
     if (warp == 0) {
         // ------------------------------------------------ TMA producer
         if (lane == 0) {
             pdl_wait();  // the operands may be written by the previous grid
+            const int col = tile * TILE;
             int stage = 0, total = 0;
             uint32_t phase = 0;
-            bool ok = true;
-            for (int t = first; ok && t < p.tiles; t += p.clusters) {
-                const int col = t * TILE;
-                for (int kb = rank; kb < p.kbs; kb += S) {
-                    if (!mbar_wait(empty0 + 8u * stage, phase ^ 1u, abort_flag)) {
-                        ok = false;
-                        break;
-                    }
-                    const uint32_t fb = full0 + 8u * stage;
-                    const uint32_t w = smem_u32(smem + stage * Cfg::STAGE_BYTES), x = w + Cfg::W_BYTES;
-                    const int k = kb * Cfg::KB;
-                    mbar_arrive_expect_tx(fb, Cfg::STAGE_BYTES);
-                    if constexpr (MODE == FS_GLU) {
-                        tma_load_3d(w, &tmW0, fb, col, k, 0);
-                        tma_load_3d(w + 16384, &tmW1, fb, col, k, 0);
-                    } else {
-                        tma_load_3d(w, &tmW0, fb, k, col, 0);
-                        tma_load_3d(w + 16384, &tmW0, fb, k + 128, col, 0);
-                    }
-                    tma_load_3d(x, &tmX, fb, k, 0, 0);
-                    tma_load_3d(x + MP * 128, &tmX, fb, k + Cfg::KB / 2, 0, 0);
-                    ++total;
-                    if (++stage == STAGES) {
-                        stage = 0;
-                        phase ^= 1u;
-                    }
+            for (int kb = rank; kb < p.kbs; kb += S) {
+                if (!mbar_wait(empty0 + 8u * stage, phase ^ 1u, abort_flag)) break;
+                const uint32_t fb = full0 + 8u * stage;
+                const uint32_t w = smem_u32(smem + stage * Cfg::STAGE_BYTES);
+                const int k = kb * Cfg::KB;
+                mbar_arrive_expect_tx(fb, Cfg::STAGE_BYTES);
+                if constexpr (MODE == FS_GLU) {
+                    tma_load_3d(w, &tmW0, fb, col, k, 0);
+                    tma_load_3d(w + 8192, &tmW1, fb, col, k, 0);
+                } else {
+                    tma_load_3d(w, &tmW0, fb, k, col, 0);
+                }
+                tma_load_3d(w + Cfg::W_BYTES, &tmX, fb, k, 0, 0);
+                ++total;
+                if (++stage == STAGES) {
+                    stage = 0;
+                    phase ^= 1u;
                 }
             }
-            // Every load issued must land before the CTA leaves.
+            // Every load issued must land before the ring is reused.
             for (int s = 0; s < STAGES && s < total; ++s) {
                 const int i = s + ((total - 1 - s) / STAGES) * STAGES;  // last k-block on slot s
                 mbar_wait(full0 + 8u * s, (uint32_t)(i / STAGES) & 1u, nullptr);
@@ -174,140 +150,98 @@ __global__ void __launch_bounds__(192, 1)
     } else if (warp == 1) {
         // ------------------------------------------------ MMA issuer
         if (lane == 0) {
-            int stage = 0, acc = 0;
-            uint32_t phase = 0, acc_phase = 0;
-            bool ok = true;
-            // Weights: MN-major, two blocks of 64 columns x 128 rows, or
-            // K-major, two chunks of 128 rows x 128 bytes.  Tokens: two
-            // K-major chunks of MP rows x 128 bytes.
-            const uint64_t w0 = MODE == FS_GLU ? umma_desc_sw128(smem_u32(smem), 16384, 1024)
+            int stage = 0;
+            uint32_t phase = 0;
+            // Weights: MN-major, two blocks of 64 columns x 64 rows, or
+            // K-major, 128 rows x 128 bytes.  Tokens: MP rows x 128 bytes.
+            const uint64_t w0 = MODE == FS_GLU ? umma_desc_sw128(smem_u32(smem), 8192, 1024)
                                                : umma_desc_sw128(smem_u32(smem), 16, 1024);
             const uint64_t x0 = umma_desc_sw128(smem_u32(smem) + Cfg::W_BYTES, 16, 1024);
             const uint32_t id = MODE == FS_GLU ? umma_idesc_f16(128, MP, true, false) : umma_idesc_i8(128, MP);
-            for (int t = first; ok && t < p.tiles; t += p.clusters) {
-                if (!mbar_wait(tempty0 + 8u * acc, acc_phase ^ 1u, abort_flag)) break;
+            for (int kb = rank; kb < p.kbs; kb += S) {
+                if (!mbar_wait(full0 + 8u * stage, phase, abort_flag)) break;
                 tc_fence_after();
-                const uint32_t d = tmem_base + (uint32_t)(acc * MP);
-                for (int kb = rank; kb < p.kbs; kb += S) {
-                    if (!mbar_wait(full0 + 8u * stage, phase, abort_flag)) {
-                        ok = false;
-                        break;
-                    }
-                    tc_fence_after();
-                    const uint64_t at = (uint64_t)((stage * Cfg::STAGE_BYTES) >> 4);
+                const uint64_t at = (uint64_t)((stage * Cfg::STAGE_BYTES) >> 4);
 #pragma unroll
-                    for (int kk = 0; kk < 8; ++kk) {
-                        const uint32_t more = (kb != rank || kk != 0) ? 1u : 0u;
-                        const uint64_t xd = x0 + at + (uint64_t)(((kk >> 2) * MP * 128 + (kk & 3) * 32) >> 4);
-                        if constexpr (MODE == FS_GLU)
-                            tc_mma_f16(d, w0 + at + (uint64_t)((kk * 2048) >> 4), xd, id, more);
-                        else
-                            tc_mma_i8(d, w0 + at + (uint64_t)(((kk >> 2) * 16384 + (kk & 3) * 32) >> 4), xd, id, more);
-                    }
-                    tc_commit(empty0 + 8u * stage);
-                    if (++stage == STAGES) {
-                        stage = 0;
-                        phase ^= 1u;
-                    }
+                for (int kk = 0; kk < 4; ++kk) {
+                    const uint32_t more = (kb != rank || kk != 0) ? 1u : 0u;
+                    const uint64_t xd = x0 + at + (uint64_t)(kk * 2);
+                    if constexpr (MODE == FS_GLU)
+                        tc_mma_f16(tmem_base, w0 + at + (uint64_t)(kk * 128), xd, id, more);
+                    else
+                        tc_mma_i8(tmem_base, w0 + at + (uint64_t)(kk * 2), xd, id, more);
                 }
-                if (!ok) break;
-                tc_commit(tfull0 + 8u * acc);
-                if (++acc == 2) {
-                    acc = 0;
-                    acc_phase ^= 1u;
+                tc_commit(empty0 + 8u * stage);
+                if (++stage == STAGES) {
+                    stage = 0;
+                    phase ^= 1u;
                 }
             }
-            tc_commit(drain_bar);
-            mbar_wait(drain_bar, 0, nullptr);
+            tc_commit(done_bar);
+            mbar_wait(done_bar, 0, nullptr);
         }
     } else {
-        // ------------------------------------------------ epilogue
         pdl_wait();  // outputs and scales may belong to the previous grid
-        const int q = warp & 3;            // TMEM lane quarter this warp may read
-        const int tid = (int)threadIdx.x - 64;
-        const int l = q * 32 + lane;       // this thread's MMA row
-        const int f = l & (TILE - 1);      // its column in the tile (gated: rows 64.. are the up projection)
-        // Where its partial sums go: part `dest`, column f - start.
+        mbar_wait(done_bar, 0, nullptr);
+        __syncwarp();
+        tc_fence_after();
+        const uint32_t src = tmem_base + ((uint32_t)(q * 32) << 16);
+#pragma unroll
+        for (int c = 0; c < MP; c += 16) tmem_ld_32x32b_x16(src + (uint32_t)c, v + c);
+        tmem_wait_ld();
+        tc_fence_before();
+    }
+
+    // ------------------------------------------------ reduction
+    __syncwarp();
+    cluster_sync();  // every CTA's ring is idle: its loads and MMAs are done
+    const int stride = (MODE == FS_GLU ? 2 : 1) * ((TILE + S - 1) / S);  // values a token and contribution
+    if (warp >= 2) {
+        const int l = q * 32 + lane;  // this thread's MMA row
+        const int f = l & (TILE - 1);  // its column in the tile (gated: rows 64.. are the up projection)
         const int dest = f * S / TILE;
         const int dstart = part_start<TILE>(dest, S), dwidth = part_start<TILE>(dest + 1, S) - dstart;
         const int at = f - dstart + (MODE == FS_GLU && l >= TILE ? dwidth : 0);
-        const int stride = (MODE == FS_GLU ? 2 : 1) * ((TILE + S - 1) / S);  // values a token and contribution
-        // This CTA's part.
-        const int pstart = part_start<TILE>(rank, S), pwidth = part_start<TILE>(rank + 1, S) - pstart;
-        const uint32_t send = mapa_shared(smem_u32(recv + rank * p.M * stride + at), (uint32_t)dest);
-        int acc = 0, i = 0;
-        uint32_t acc_phase = 0;
-        for (int t = first; t < p.tiles; t += p.clusters, ++i) {
-            const int b = i % RB;
-            bool ok = mbar_wait(tfull0 + 8u * acc, acc_phase, abort_flag);
-            ok = __all_sync(0xffffffffu, ok);
-            if (!ok) break;
-            tc_fence_after();
-            float v[MP];
-            const uint32_t src = tmem_base + ((uint32_t)(q * 32) << 16) + (uint32_t)(acc * MP);
+        const uint32_t to = mapa_shared(smem_u32(smem) + (uint32_t)(rank * p.M * stride + at) * 4u, (uint32_t)dest);
 #pragma unroll
-            for (int c = 0; c < MP; c += 16) tmem_ld_32x32b_x16(src + (uint32_t)c, v + c);
-            tmem_wait_ld();
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(tempty0 + 8u * acc);
-            if (++acc == 2) {
-                acc = 0;
-                acc_phase ^= 1u;
-            }
-            // The owners have read this buffer's last contents.
-            if (i >= RB) ok = mbar_wait<true>(credit0 + 8u * b, (uint32_t)(i / RB - 1) & 1u, abort_flag);
-            ok = __all_sync(0xffffffffu, ok);
-            if (!ok) break;
-            const uint32_t to = send + (uint32_t)(b * Cfg::RECV_FLOATS * 4);
-#pragma unroll
-            for (int m = 0; m < MP; ++m)
-                if (m < p.M) st_shared_cluster_f32(to + (uint32_t)(m * stride * 4), v[m]);
-            __syncwarp();
-            if (lane < S) mbar_arrive_cluster(recv0 + 8u * b, (uint32_t)lane);
-            ok = mbar_wait<true>(recv0 + 8u * b, (uint32_t)(i / RB) & 1u, abort_flag);
-            ok = __all_sync(0xffffffffu, ok);
-            if (!ok) break;
-            // This CTA's columns: the contributions in CTA order.
-            const float* r = recv + b * Cfg::RECV_FLOATS;
-            for (int e = tid; e < p.M * pwidth; e += 128) {
-                const int m = e / pwidth, c = e - m * pwidth;
-                const long long col = (long long)t * TILE + pstart + c;
-                if (col >= p.N) continue;
-                if constexpr (MODE == FS_GLU) {
-                    float g = 0.f, u = 0.f;
-                    for (int s = 0; s < S; ++s) {
-                        const float* x = r + (s * p.M + m) * stride + c;
-                        g += x[0];
-                        u += x[pwidth];
-                    }
-                    p.H[m * p.ldh + col] = __float2half_rn(act_value_rt(p.act, g) * u);
-                    if (p.G) {
-                        p.G[m * p.ldg + col] = __float2half_rn(g);
-                        p.U[m * p.ldu + col] = __float2half_rn(u);
-                    }
-                } else {
-                    int sum = 0;
-                    for (int s = 0; s < S; ++s) sum += __float_as_int(r[(s * p.M + m) * stride + c]);
-                    float o = (float)sum * p.sa[m] * p.sb[col];
-                    if (p.bias) o += __half2float(p.bias[col]);
-                    if (p.c_f16)
-                        static_cast<__half*>(p.C)[m * p.ldc + col] = __float2half_rn(o);
-                    else
-                        static_cast<float*>(p.C)[m * p.ldc + col] = o;
-                }
-            }
-            epilogue_sync();  // the part is read: the senders may reuse the buffer
-            if (tid < S) mbar_arrive_cluster(credit0 + 8u * b, (uint32_t)tid);
-        }
+        for (int m = 0; m < MP; ++m)
+            if (m < p.M) st_shared_cluster_f32(to + (uint32_t)(m * stride * 4), v[m]);
     }
-
     __syncwarp();
-    tc_fence_before();
-    cluster_sync();  // no CTA leaves while a peer may still write to it
+    cluster_sync();  // the contributions are in; nothing remote happens after this
     if (warp == 1) {
         tc_fence_after();
         tmem_dealloc<1>(tmem_base, Cfg::TMEM_COLS);
+    }
+    if (*abort_flag) return;
+    const float* r = reinterpret_cast<const float*>(smem);
+    const int pstart = part_start<TILE>(rank, S), pwidth = part_start<TILE>(rank + 1, S) - pstart;
+    for (int e = (int)threadIdx.x; e < p.M * pwidth; e += 192) {
+        const int m = e / pwidth, c = e - m * pwidth;
+        const long long col = (long long)tile * TILE + pstart + c;
+        if (col >= p.N) continue;
+        if constexpr (MODE == FS_GLU) {
+            float g = 0.f, u = 0.f;
+            for (int s = 0; s < S; ++s) {
+                const float* x = r + (s * p.M + m) * stride + c;
+                g += x[0];
+                u += x[pwidth];
+            }
+            p.H[m * p.ldh + col] = __float2half_rn(act_value_rt(p.act, g) * u);
+            if (p.G) {
+                p.G[m * p.ldg + col] = __float2half_rn(g);
+                p.U[m * p.ldu + col] = __float2half_rn(u);
+            }
+        } else {
+            int sum = 0;
+            for (int s = 0; s < S; ++s) sum += __float_as_int(r[(s * p.M + m) * stride + c]);
+            float o = (float)sum * p.sa[m] * p.sb[col];
+            if (p.bias) o += __half2float(p.bias[col]);
+            if (p.c_f16)
+                static_cast<__half*>(p.C)[m * p.ldc + col] = __float2half_rn(o);
+            else
+                static_cast<float*>(p.C)[m * p.ldc + col] = o;
+        }
     }
 }
 
@@ -327,58 +261,31 @@ bool fs_map(CUtensorMap* m, const void* base, bool i8, long long rows, long long
 
 constexpr int kMaxSplit = 8;
 
-// Clusters of S CTAs that device `dev` holds at once; also sets the kernel's
-// shared-memory limit there.  Asked once per device, kernel and S.
 template <int MODE, int MP>
-int fs_clusters(int dev, int S) {
-    static int cache[64][kMaxSplit + 1] = {{0}};
-    int& v = cache[dev & 63][S];
-    if (v == 0) {
-        using Cfg = FsCfg<MODE, MP>;
-        auto kern = ff_skinny_kernel<MODE, MP>;
-        if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)Cfg::SMEM_BYTES) != cudaSuccess)
-            return 0;
-        cudaLaunchConfig_t cfg = {};
-        cudaLaunchAttribute attr[1];
-        attr[0].id = cudaLaunchAttributeClusterDimension;
-        attr[0].val.clusterDim.x = S;
-        attr[0].val.clusterDim.y = 1;
-        attr[0].val.clusterDim.z = 1;
-        cfg.blockDim = dim3(192);
-        cfg.dynamicSmemBytes = Cfg::SMEM_BYTES;
-        cfg.attrs = attr;
-        cfg.numAttrs = 1;
-        cfg.gridDim = dim3(device_sm_count(dev) / S * S);
-        int n = 0;
-        if (cudaOccupancyMaxActiveClusters(&n, kern, &cfg) != cudaSuccess || n <= 0) {
-            cudaGetLastError();
-            return 0;
-        }
-        v = n;
-    }
-    return v;
+bool fs_prepare(int dev) {
+    static bool done[64] = {false};
+    bool& d = done[dev & 63];
+    if (!d)
+        d = cudaFuncSetAttribute(ff_skinny_kernel<MODE, MP>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                 (int)FsCfg<MODE, MP>::SMEM_BYTES) == cudaSuccess;
+    return d;
 }
 
 template <int MODE, int MP>
-pax_status_t launch_skinny(const CUtensorMap& w0, const CUtensorMap& w1, const CUtensorMap& x, FsParams& p,
+pax_status_t launch_skinny(const CUtensorMap& w0, const CUtensorMap& w1, const CUtensorMap& x, const FsParams& p,
                            cudaStream_t stream) {
     using Cfg = FsCfg<MODE, MP>;
-    const int dev = current_device();
-    // The busiest cluster's k-blocks, and about half a k-block's time to
-    // reduce a tile.
-    int S = 0;
-    double best = 0;
-    for (int s = 1; s <= kMaxSplit && s <= p.kbs; ++s) {
-        const int n = fs_clusters<MODE, MP>(dev, s);
-        if (n <= 0) continue;
-        const double cost = ((p.tiles + n - 1) / n) * ((p.kbs + s - 1) / s + 0.5);
-        if (S == 0 || cost < best) {
-            S = s;
-            best = cost;
-            p.clusters = p.tiles < n ? p.tiles : n;
-        }
-    }
-    if (S == 0) return PAX_ERR_CUDA;
+    const int dev = current_device(), sms = device_sm_count(dev);
+    if (!fs_prepare<MODE, MP>(dev)) return PAX_ERR_CUDA;
+    const long long tiles = (p.N + Cfg::TILE - 1) / Cfg::TILE;
+    // As many CTAs as are resident at once, with at least four k-blocks each.
+    // A CTA that has to wait for another's end costs more than the finer
+    // split gains: 1x2048x5504 in 86 / 172 / 258 / 344 CTAs takes 15.4 / 13.5
+    // / 13.6 / 17.7 us, 24x4096x11264 in 176 / 352 / 704 takes 35.6 / 42.9 /
+    // 45.0.
+    int S = 1;
+    while (S < kMaxSplit && tiles * (S + 1) <= 2 * sms && p.kbs >= 4 * (S + 1)) ++S;
+    if (tiles * S > 0x7fffffffLL) return PAX_ERR_UNSUPPORTED;
     cudaLaunchConfig_t cfg = {};
     cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -387,7 +294,7 @@ pax_status_t launch_skinny(const CUtensorMap& w0, const CUtensorMap& w1, const C
     attr[1].val.clusterDim.x = S;
     attr[1].val.clusterDim.y = 1;
     attr[1].val.clusterDim.z = 1;
-    cfg.gridDim = dim3(p.clusters * S);
+    cfg.gridDim = dim3((unsigned)(tiles * S));
     cfg.blockDim = dim3(192);
     cfg.dynamicSmemBytes = Cfg::SMEM_BYTES;
     cfg.stream = stream;
@@ -397,7 +304,7 @@ pax_status_t launch_skinny(const CUtensorMap& w0, const CUtensorMap& w1, const C
 }
 
 template <int MODE>
-pax_status_t launch_tokens(const CUtensorMap& w0, const CUtensorMap& w1, const CUtensorMap& x, FsParams& p,
+pax_status_t launch_tokens(const CUtensorMap& w0, const CUtensorMap& w1, const CUtensorMap& x, const FsParams& p,
                            cudaStream_t stream) {
     if (p.M <= 16) return launch_skinny<MODE, 16>(w0, w1, x, p, stream);
     if (p.M <= 32) return launch_skinny<MODE, 32>(w0, w1, x, p, stream);
@@ -419,14 +326,13 @@ bool glu_skinny_ok(const GluProblem& q) {
 
 pax_status_t glu_skinny(const GluProblem& q, cudaStream_t stream) {
     CUtensorMap wg, wu, x;
-    if (!fs_map(&wg, q.Wg, false, q.D, q.F, q.ldwg, 64, 128) || !fs_map(&wu, q.Wu, false, q.D, q.F, q.ldwu, 64, 128) ||
+    if (!fs_map(&wg, q.Wg, false, q.D, q.F, q.ldwg, 64, 64) || !fs_map(&wu, q.Wu, false, q.D, q.F, q.ldwu, 64, 64) ||
         !fs_map(&x, q.X, false, q.M, q.D, q.ldx, 64, padded(q.M)))
         return PAX_ERR_CUDA;
     FsParams p = {};
     p.M = (int)q.M;
     p.N = (int)q.F;
-    p.tiles = (int)((q.F + 63) / 64);
-    p.kbs = (int)((q.D + 127) / 128);
+    p.kbs = (int)((q.D + 63) / 64);
     p.H = q.H, p.G = q.G, p.U = q.U;
     p.ldh = q.ldh, p.ldg = q.ldg, p.ldu = q.ldu;
     p.act = q.act;
@@ -444,8 +350,7 @@ pax_status_t gemm_i8_skinny(const I8Problem& q, cudaStream_t stream) {
     FsParams p = {};
     p.M = (int)q.M;
     p.N = (int)q.N;
-    p.tiles = (int)((q.N + 127) / 128);
-    p.kbs = (int)((q.K + 255) / 256);
+    p.kbs = (int)((q.K + 127) / 128);
     p.C = q.C;
     p.ldc = q.ldc;
     p.sa = q.a_scale, p.sb = q.b_scale, p.bias = q.bias;

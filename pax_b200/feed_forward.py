@@ -10,7 +10,6 @@ a caller that passes ``stream`` orders its own use of the output after it.
 """
 from __future__ import annotations
 
-import contextlib
 import ctypes
 from enum import IntEnum
 
@@ -37,32 +36,34 @@ def _activation(a) -> int:
     return int(Activation(a))
 
 
-def _matrix(t: torch.Tensor, name: str, shape: tuple, dtypes: tuple, device: torch.device | None) -> int:
+def _matrix(t: torch.Tensor, name: str, rows: int, cols: int, dtypes: tuple, device: torch.device) -> int:
     """Checks an operand and returns its leading dimension (elements)."""
     if not isinstance(t, torch.Tensor):
         raise TypeError(f"{name} must be a tensor")
     if t.dtype not in dtypes:
         raise TypeError(f"{name} must be {' or '.join(str(d).removeprefix('torch.') for d in dtypes)}")
-    if tuple(t.shape) != shape:
-        raise ValueError(f"{name} has shape {tuple(t.shape)}, expected {shape}")
-    if device is not None and t.device != device:
+    if t.shape != (rows, cols):
+        raise ValueError(f"{name} has shape {tuple(t.shape)}, expected {(rows, cols)}")
+    if t.device != device:
         raise ValueError(f"{name} is on {t.device}, expected {device}")
-    if t.numel() == 0:
+    s0, s1 = t.stride()
+    if rows > 1 and s1 == 1 and s0 >= cols > 0:
+        return s0
+    if rows == 0 or cols == 0:
         return 0
-    rows, cols = shape
-    if cols > 1 and t.stride(1) != 1:
+    if cols > 1 and s1 != 1:
         raise ValueError(f"{name} must be a 2-D tensor with unit column stride")
     if rows == 1:  # the pitch of one row is never used
         return 0
-    if t.stride(0) < cols:  # expanded or overlapping rows
+    if s0 < cols:  # expanded or overlapping rows
         raise ValueError(f"{name} must have rows that do not overlap")
-    return t.stride(0)
+    return s0
 
 
 def _vector(t: torch.Tensor, name: str, n: int, dtype: torch.dtype, device: torch.device) -> None:
     if not isinstance(t, torch.Tensor) or t.dtype != dtype:
         raise TypeError(f"{name} must be a {str(dtype).removeprefix('torch.')} tensor")
-    if tuple(t.shape) != (n,):
+    if t.shape != (n,):
         raise ValueError(f"{name} has shape {tuple(t.shape)}, expected ({n},)")
     if t.device != device:
         raise ValueError(f"{name} is on {t.device}, expected {device}")
@@ -73,7 +74,7 @@ def _vector(t: torch.Tensor, name: str, n: int, dtype: torch.dtype, device: torc
 def _dims(t, name: str) -> tuple:
     if not isinstance(t, torch.Tensor) or t.dim() != 2:
         raise ValueError(f"{name} must be a 2-D tensor")
-    return tuple(t.shape)
+    return t.shape
 
 
 class _Call:
@@ -82,34 +83,43 @@ class _Call:
     after them can overlap the call, and stay reserved for the caller's
     current stream as well."""
 
+    __slots__ = ("device", "other", "raw")
+
     def __init__(self, device: torch.device, stream: torch.cuda.Stream | None):
         if device.type != "cuda":
             raise ValueError("tensors must be on a CUDA device")
-        if stream is not None and stream.device != device:
-            raise ValueError(f"stream is on {stream.device}, expected {device}")
         self.device = device
-        self.current = torch.cuda.current_stream(device)
-        self.stream = stream if stream is not None else self.current
-        self.other = self.stream != self.current
-
-    def scope(self):
-        return torch.cuda.stream(self.stream) if self.other else contextlib.nullcontext()
+        self.other = None
+        if stream is None:
+            self.raw = torch._C._cuda_getCurrentRawStream(device.index)
+        else:
+            if stream.device != device:
+                raise ValueError(f"stream is on {stream.device}, expected {device}")
+            self.raw = stream.cuda_stream
+            if stream != torch.cuda.current_stream(device):
+                self.other = stream
 
     def empty(self, shape, dtype, scratch=False) -> torch.Tensor:
-        with self.scope():
+        if self.other is None:
+            return torch.empty(shape, dtype=dtype, device=self.device)
+        with torch.cuda.stream(self.other):
             t = torch.empty(shape, dtype=dtype, device=self.device)
-        if self.other and not scratch:
-            t.record_stream(self.current)
+        if not scratch:
+            t.record_stream(torch.cuda.current_stream(self.device))
         return t
 
     def run(self, name: str, *args) -> None:
-        with torch.cuda.device(self.device):
-            st = getattr(_lib.get(), name)(*args, ctypes.c_void_p(self.stream.cuda_stream))
+        fn = getattr(_lib.get(), name)
+        if torch.cuda.current_device() == self.device.index:
+            st = fn(*args, self.raw)
+        else:
+            with torch.cuda.device(self.device):
+                st = fn(*args, self.raw)
         if st != 0:
             raise PaxError(st, name)
 
 
-_F16 = (torch.float16,)
+_F16, _I8, _OUT = (torch.float16,), (torch.int8,), tuple(_DT)
 
 
 def glu(X: torch.Tensor, Wg: torch.Tensor, Wu: torch.Tensor, *, activation="silu", save: bool = False,
@@ -129,23 +139,19 @@ def glu(X: torch.Tensor, Wg: torch.Tensor, Wu: torch.Tensor, *, activation="silu
     if (G is None) != (U is None):
         raise ValueError("G and U go together")
     dev = X.device
-    d = _lib.GluDesc()
-    d.M, d.D, d.F, d.act = M, D, F, act
-    d.ldx = _matrix(X, "X", (M, D), _F16, dev)
-    d.ldwg = _matrix(Wg, "Wg", (D, F), _F16, dev)
-    d.ldwu = _matrix(Wu, "Wu", (D, F), _F16, dev)
-    for t, name in ((out, "out"), (G, "G"), (U, "U")):
-        if t is not None:
-            _matrix(t, name, (M, F), _F16, dev)
+    ldx = _matrix(X, "X", M, D, _F16, dev)
+    ldwg, ldwu = _matrix(Wg, "Wg", D, F, _F16, dev), _matrix(Wu, "Wu", D, F, _F16, dev)
+    ldh = _matrix(out, "out", M, F, _F16, dev) if out is not None else F
+    ldg = ldu = F
+    if G is not None:
+        ldg, ldu = _matrix(G, "G", M, F, _F16, dev), _matrix(U, "U", M, F, _F16, dev)
     call = _Call(dev, stream)
     H = out if out is not None else call.empty((M, F), torch.float16)
     if save and G is None:
         G, U = call.empty((M, F), torch.float16), call.empty((M, F), torch.float16)
-    d.X, d.Wg, d.Wu, d.H = X.data_ptr(), Wg.data_ptr(), Wu.data_ptr(), H.data_ptr()
-    d.ldh = _matrix(H, "out", (M, F), _F16, dev)
-    if G is not None:
-        d.G, d.U = G.data_ptr(), U.data_ptr()
-        d.ldg, d.ldu = _matrix(G, "G", (M, F), _F16, dev), _matrix(U, "U", (M, F), _F16, dev)
+    g, u = (0, 0) if G is None else (G.data_ptr(), U.data_ptr())
+    d = _lib.GluDesc(X.data_ptr(), Wg.data_ptr(), Wu.data_ptr(), H.data_ptr(), g, u, M, D, F, ldx, ldwg, ldwu, ldh, ldg,
+                     ldu, act)
     call.run("pax_glu_ex", ctypes.byref(d))
     return H if G is None else (H, G, U)
 
@@ -167,8 +173,7 @@ def glu_backward(dH: torch.Tensor, X: torch.Tensor, Wg: torch.Tensor, Wu: torch.
     M, D = _dims(X, "X")
     _, F = _dims(Wg, "Wg")
     dev = X.device
-    d = _lib.GluGradDesc()
-    d.M, d.D, d.F, d.act = M, D, F, _activation(activation)
+    act = _activation(activation)
     if (dWg is None) != (dWu is None):
         raise ValueError("dWg and dWu go together")
     if dWg is not None:
@@ -181,28 +186,22 @@ def glu_backward(dH: torch.Tensor, X: torch.Tensor, Wg: torch.Tensor, Wu: torch.
         raise TypeError("weight gradients must be float32 or float16")
     if accumulate and (dWg is None or dW_dtype != torch.float32):
         raise ValueError("accumulate needs given float32 dWg and dWu")
-    for t, name, shape in ((dH, "dH", (M, F)), (X, "X", (M, D)), (Wg, "Wg", (D, F)), (Wu, "Wu", (D, F)), (G, "G", (M, F)),
-                           (U, "U", (M, F))):
-        setattr(d, "ld" + name.lower(), _matrix(t, name, shape, _F16, dev))
-        setattr(d, name, t.data_ptr())
-    for t, name, shape, dt in ((dX, "dX", (M, D), _F16), (dWg, "dWg", (D, F), (dW_dtype,)),
-                               (dWu, "dWu", (D, F), (dW_dtype,)), (dG, "dG", (M, F), _F16), (dU, "dU", (M, F), _F16)):
-        if t is not None:
-            _matrix(t, name, shape, dt, dev)
+    ins = ((dH, "dH", M, F), (X, "X", M, D), (Wg, "Wg", D, F), (Wu, "Wu", D, F), (G, "G", M, F), (U, "U", M, F))
+    lds = [_matrix(t, name, r, c, _F16, dev) for t, name, r, c in ins]
+    for t, name, r, c, dt in ((dG, "dG", M, F, _F16), (dU, "dU", M, F, _F16), (dX, "dX", M, D, _F16),
+                              (dWg, "dWg", D, F, (dW_dtype,)), (dWu, "dWu", D, F, (dW_dtype,))):
+        lds.append(c if t is None else _matrix(t, name, r, c, dt, dev))
     call = _Call(dev, stream)
     if need_dX and dX is None:
         dX = call.empty((M, D), torch.float16)
     if need_dW and dWg is None:
         dWg, dWu = call.empty((D, F), dW_dtype), call.empty((D, F), dW_dtype)
-    dG = dG if dG is not None else call.empty((M, F), torch.float16, scratch=True)
-    dU = dU if dU is not None else call.empty((M, F), torch.float16, scratch=True)
-    for t, name, shape in ((dG, "dG", (M, F)), (dU, "dU", (M, F)), (dX, "dX", (M, D)), (dWg, "dWg", (D, F)),
-                           (dWu, "dWu", (D, F))):
-        if t is not None:
-            setattr(d, "ld" + name.lower(), _matrix(t, name, shape, (t.dtype,), dev))
-            setattr(d, name, t.data_ptr())
-    d.dw_dtype = int(_DT[dW_dtype])
-    d.accumulate = int(accumulate)
+    if dG is None:
+        dG = call.empty((M, F), torch.float16, scratch=True)
+    if dU is None:
+        dU = call.empty((M, F), torch.float16, scratch=True)
+    d = _lib.GluGradDesc(*(0 if t is None else t.data_ptr() for t in (dH, X, Wg, Wu, G, U, dG, dU, dX, dWg, dWu)), M, D, F,
+                         *lds, _DT[dW_dtype], accumulate, act)
     call.run("pax_glu_backward_ex", ctypes.byref(d))
     return dX, dWg, dWu
 
@@ -217,17 +216,14 @@ def quantize_rows(X: torch.Tensor, *, out: torch.Tensor | None = None, scale: to
     """
     M, K = _dims(X, "X")
     dev = X.device
-    ldx = _matrix(X, "X", (M, K), _F16, dev)
-    if out is not None:
-        _matrix(out, "out", (M, K), (torch.int8,), dev)
+    ldx = _matrix(X, "X", M, K, _F16, dev)
+    ldq = _matrix(out, "out", M, K, _I8, dev) if out is not None else K
     if scale is not None:
         _vector(scale, "scale", M, torch.float32, dev)
     call = _Call(dev, stream)
     Q = out if out is not None else call.empty((M, K), torch.int8)
     s = scale if scale is not None else call.empty((M,), torch.float32)
-    ldq = _matrix(Q, "out", (M, K), (torch.int8,), dev)
-    call.run("pax_quantize_rows", ctypes.c_void_p(X.data_ptr()), ldx, ctypes.c_void_p(Q.data_ptr()), ldq,
-             ctypes.c_void_p(s.data_ptr()), M, K)
+    call.run("pax_quantize_rows", X.data_ptr(), ldx, Q.data_ptr(), ldq, s.data_ptr(), M, K)
     return Q, s
 
 
@@ -244,25 +240,20 @@ def gemm_i8(A: torch.Tensor, B: torch.Tensor, a_scale: torch.Tensor, b_scale: to
     M, K = _dims(A, "A")
     N, _ = _dims(B, "B")
     dev = A.device
-    d = _lib.GemmI8Desc()
-    d.M, d.N, d.K = M, N, K
-    i8 = (torch.int8,)
-    d.lda, d.ldb = _matrix(A, "A", (M, K), i8, dev), _matrix(B, "B", (N, K), i8, dev)
+    lda, ldb = _matrix(A, "A", M, K, _I8, dev), _matrix(B, "B", N, K, _I8, dev)
     _vector(a_scale, "a_scale", M, torch.float32, dev)
     _vector(b_scale, "b_scale", N, torch.float32, dev)
     if bias is not None:
         _vector(bias, "bias", N, torch.float16, dev)
+    ldc = N
     if out is not None:
-        _matrix(out, "out", (M, N), tuple(_DT), dev)
+        ldc = _matrix(out, "out", M, N, _OUT, dev)
+        out_dtype = out.dtype
     elif out_dtype not in _DT:
         raise TypeError("out_dtype must be float32 or float16")
     call = _Call(dev, stream)
     C = out if out is not None else call.empty((M, N), out_dtype)
-    d.A, d.B, d.C = A.data_ptr(), B.data_ptr(), C.data_ptr()
-    d.ldc = _matrix(C, "out", (M, N), tuple(_DT), dev)
-    d.a_scale, d.b_scale = a_scale.data_ptr(), b_scale.data_ptr()
-    if bias is not None:
-        d.bias = bias.data_ptr()
-    d.c_dtype = int(_DT[C.dtype])
+    d = _lib.GemmI8Desc(A.data_ptr(), B.data_ptr(), C.data_ptr(), a_scale.data_ptr(), b_scale.data_ptr(),
+                        0 if bias is None else bias.data_ptr(), M, N, K, lda, ldb, ldc, _DT[out_dtype])
     call.run("pax_gemm_i8_ex", ctypes.byref(d))
     return C
