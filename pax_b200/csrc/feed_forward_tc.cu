@@ -25,32 +25,76 @@ int up(long long a, int b) { return (int)((a + b - 1) / b); }
 // gemm_tc.cuh, where 16 measured best at every shape).
 constexpr int kGroupM = 16;
 
-template <int ACT>
-pax_status_t launch_glu(const FfMaps& maps, const FfParams& p, cudaStream_t stream) {
-    const int most = ff_units<FF_GLU, ACT, __half>(current_device());
+// Which tile width: the time in k-blocks of the narrow tile, about 0.36 us
+// each.  A k-block of the wide tile takes 1.62 of them for twice the work;
+// its epilogue, not overlapped, about 12 (measured over K = 64 to 2048 on
+// 777 x 4104 .. 9472; the last epilogue of a narrow tile about 8).
+// 4096x4096x11264 takes 608-628 us with the wide tile and 646 with the
+// narrow one, 777x1024x4736 (148 narrow tiles) 27.2 and 17.3 us.
+constexpr double kWideBlock = 1.62, kWideEpilogue = 12.0, kLastEpilogue = 8.0;
+
+double tile_cost(int w, int kbs) { return w == 2 ? kbs * kWideBlock + kWideEpilogue : kbs; }
+
+int rounds(long long tiles, int units) { return (int)((tiles + units - 1) / units); }
+
+template <int ACT, int W>
+pax_status_t launch_glu_w(const FfMaps& maps, FfParams& p, cudaStream_t stream) {
+    const int most = ff_units<FF_GLU, ACT, __half, W>(current_device());
     if (most <= 0) return PAX_ERR_CUDA;
+    p.tiles_n = up(p.N, 128 * W);
     const long long tiles = (long long)p.tiles_m * p.tiles_n;
-    return ff_launch<FF_GLU, ACT, __half>(maps, p, (int)(tiles < most ? tiles : most), stream);
+    return ff_launch<FF_GLU, ACT, __half, W>(maps, p, (int)(tiles < most ? tiles : most), stream);
+}
+template <int ACT>
+pax_status_t launch_glu(const FfMaps& maps, FfParams& p, cudaStream_t stream) {
+    const int units = ff_units<FF_GLU, ACT, __half, 1>(current_device());
+    if (units <= 0) return PAX_ERR_CUDA;
+    const double t1 = rounds((long long)p.tiles_m * up(p.N, 128), units) * tile_cost(1, p.kbs) + kLastEpilogue;
+    const double t2 = rounds((long long)p.tiles_m * up(p.N, 256), units) * tile_cost(2, p.kbs);
+    return t2 < t1 ? launch_glu_w<ACT, 2>(maps, p, stream) : launch_glu_w<ACT, 1>(maps, p, stream);
 }
 
-template <typename OutT>
-pax_status_t launch_back(const FfMaps& maps, FfParams& p, cudaStream_t stream) {
-    const int most = ff_units<FF_BACK, 0, OutT>(current_device());
+template <typename OutT, int W>
+pax_status_t launch_back_w(const FfMaps& maps, FfParams& p, cudaStream_t stream) {
+    const int most = ff_units<FF_BACK, 0, OutT, W>(current_device());
     if (most <= 0) return PAX_ERR_CUDA;
+    p.tiles_n = up(p.D, 256 * W);
+    p.wt_n = up(p.F, 256 * W);
+    p.nx = p.nx ? p.tiles_m * p.tiles_n : 0;
+    p.nw = p.nw ? p.wt_m * 2 * p.wt_n : 0;
     const long long items = (long long)p.nx + p.nw;
     const int units = (int)(items < most ? items : most);
     p.x_rem = p.nx % units;
     p.w_extra = 0;
     if (p.x_rem > 0 && p.nw > 0) p.w_extra = (p.kbs + p.kbs_w / 2) / p.kbs_w;
-    return ff_launch<FF_BACK, 0, OutT>(maps, p, units, stream);
+    return ff_launch<FF_BACK, 0, OutT, W>(maps, p, units, stream);
+}
+template <typename OutT>
+pax_status_t launch_back(const FfMaps& maps, FfParams& p, cudaStream_t stream) {
+    const int units = ff_units<FF_BACK, 0, OutT, 1>(current_device());
+    if (units <= 0) return PAX_ERR_CUDA;
+    // The weight gradients fill up what dX's tiles leave uneven; a launch
+    // ends no earlier than its longest tile.
+    double t[3];
+    for (int w = 1; w <= 2; ++w) {
+        const double x = p.nx ? tile_cost(w, p.kbs) : 0, y = p.nw ? tile_cost(w, p.kbs_w) : 0;
+        const long long nx = p.nx ? (long long)p.tiles_m * up(p.D, 256 * w) : 0;
+        const long long nw = p.nw ? 2LL * p.wt_m * up(p.F, 256 * w) : 0;
+        double even = p.nw ? (nx * x + nw * y) / units + 0.5 * y : rounds(nx, units) * x;
+        if (even < x) even = x;
+        if (even < y) even = y;
+        t[w] = even + (w == 1 ? kLastEpilogue : 0);
+    }
+    return t[2] < t[1] ? launch_back_w<OutT, 2>(maps, p, stream) : launch_back_w<OutT, 1>(maps, p, stream);
 }
 
 template <typename OutT>
-pax_status_t launch_i8(const FfMaps& maps, const FfParams& p, cudaStream_t stream) {
-    const int most = ff_units<FF_I8, 0, OutT>(current_device());
+pax_status_t launch_i8(const FfMaps& maps, FfParams& p, cudaStream_t stream) {
+    const int most = ff_units<FF_I8, 0, OutT, 1>(current_device());
     if (most <= 0) return PAX_ERR_CUDA;
+    p.tiles_n = up(p.N, 256);
     const long long tiles = (long long)p.tiles_m * p.tiles_n;
-    return ff_launch<FF_I8, 0, OutT>(maps, p, (int)(tiles < most ? tiles : most), stream);
+    return ff_launch<FF_I8, 0, OutT, 1>(maps, p, (int)(tiles < most ? tiles : most), stream);
 }
 
 bool tiles_ok(long long a, long long b) { return a * b <= 0x3fffffffLL; }
@@ -79,7 +123,6 @@ pax_status_t glu_tc(const GluProblem& q, cudaStream_t stream) {
     p.M = (int)q.M;
     p.N = (int)q.F;
     p.tiles_m = up(q.M, 256);
-    p.tiles_n = up(q.F, 128);
     p.kbs = up(q.D, 64);
     p.group_m = kGroupM;
     p.save = q.G != nullptr;
@@ -121,15 +164,13 @@ pax_status_t glu_back_tc(const GluGradProblem& q, cudaStream_t stream) {
     p.F = (int)q.F;
     p.N = p.D;
     p.tiles_m = up(q.M, 256);
-    p.tiles_n = up(q.D, 256);
     p.half_kbs = up(q.F, 64);
     p.kbs = 2 * p.half_kbs;
     p.group_m = kGroupM;
     p.wt_m = up(q.D, 256);
-    p.wt_n = up(q.F, 256);
     p.kbs_w = up(q.M, 64);
-    p.nx = q.dX ? p.tiles_m * p.tiles_n : 0;
-    p.nw = q.dWg ? p.wt_m * 2 * p.wt_n : 0;
+    p.nx = q.dX != nullptr;  // counted once the tile width is chosen
+    p.nw = q.dWg != nullptr;
     p.accumulate = q.accumulate;
     return q.dw_f16 ? launch_back<__half>(maps, p, stream) : launch_back<float>(maps, p, stream);
 }
@@ -153,7 +194,6 @@ pax_status_t gemm_i8_tc(const I8Problem& q, cudaStream_t stream) {
     p.M = (int)q.M;
     p.N = (int)q.N;
     p.tiles_m = up(q.M, 256);
-    p.tiles_n = up(q.N, 256);
     p.kbs = up(q.K, 128);
     p.group_m = kGroupM;
     p.C = q.C;
@@ -161,8 +201,6 @@ pax_status_t gemm_i8_tc(const I8Problem& q, cudaStream_t stream) {
     p.sa = q.a_scale;
     p.sb = q.b_scale;
     p.bias = q.bias;
-    p.sb_vec = (reinterpret_cast<uintptr_t>(q.b_scale) & 15u) == 0;
-    p.bias_vec = (reinterpret_cast<uintptr_t>(q.bias) & 15u) == 0;
     return q.c_f16 ? launch_i8<__half>(maps, p, stream) : launch_i8<float>(maps, p, stream);
 }
 

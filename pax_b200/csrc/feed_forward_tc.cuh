@@ -8,11 +8,10 @@
 //            launch
 //   FF_I8    C = (A.B^T) * sa * sb (+ bias), 8-bit integers
 //
-// A CTA pair (cluster of two, cta_group::2) computes 256 x 256 accumulator
-// tiles; each CTA stages 128 rows of A and 128 columns of B per 128-byte
-// k-block (64 fp16 or 128 int8) in a six-slot ring and holds its 128 rows of
-// two accumulators (all 512 TMEM columns), so that the epilogue of one tile
-// runs under the main loop of the next.
+// A CTA pair (cluster of two, cta_group::2) computes accumulator tiles of 256
+// rows and 256 or 512 columns; each CTA stages 128 rows of A and 128 or 256
+// columns of B per 128-byte k-block (64 fp16 or 128 int8) in a ring and holds
+// its 128 rows of the accumulators in TMEM (FfCfg).
 //
 // The gated product needs G and U of the same element in one thread.  The
 // even CTA stages 128 columns of Wg and the odd CTA the same 128 columns of
@@ -65,7 +64,7 @@ struct FfParams {
     long long ldc;
     const float *sa, *sb;
     const __half* bias;
-    int c_tma, sb_vec, bias_vec;
+    int c_tma;
 };
 
 struct FfItem {
@@ -120,32 +119,48 @@ __host__ __device__ __forceinline__ bool ff_item(const FfParams& p, int unit, in
     }
 }
 
+// Tile widths.  W = 1: 256 accumulator columns a tile, two accumulators in
+// TMEM, so that a tile's epilogue runs under the next one's main loop.
+// W = 2: 512 columns as two MMAs per k-step that share A, one accumulator in
+// all of TMEM.  It stages 48 KB for twice the MMAs instead of 2 x 32 KB, and
+// shared-memory traffic is what bounds the main loop, but its epilogue is
+// exposed.
+//
+// The 8-bit product (W = 1 only) gives one slot of its ring to tables of
+// scales and bias in shared memory, one per epilogue warp: read from global
+// memory in the epilogue they took longer than a main loop of K = 2048.
+template <int MODE, int W>
 struct FfCfg {
-    static constexpr int STAGES = 6;
+    static constexpr int STAGES = W == 2 ? 4 : MODE == FF_I8 ? 5 : 6;
     static constexpr uint32_t OP_BYTES = 128 * 128;         // 128 rows or columns, 128 bytes of k
-    static constexpr uint32_t STAGE_BYTES = 2 * OP_BYTES;
+    static constexpr uint32_t A_BYTES = OP_BYTES, B_BYTES = W * OP_BYTES;
+    static constexpr uint32_t STAGE_BYTES = A_BYTES + B_BYTES;
+    static constexpr int ACCS = W == 2 ? 1 : 2;             // accumulators in TMEM
     static constexpr int EPI_WARPS = 8;
     static constexpr int THREADS = 64 + 32 * EPI_WARPS;
     static constexpr uint32_t STG_BYTES = 32 * 128;         // staging, per epilogue warp
+    static constexpr uint32_t TAB_BYTES = MODE == FF_I8 ? 2 * 128 * 4 : 0;  // per epilogue warp
     static constexpr uint32_t NUM_BARS = 2 * STAGES + 6;    // full, empty, tfull[2], tempty[2], drain, report
-    static constexpr size_t SMEM_BYTES =
-        1024 + (size_t)STAGES * STAGE_BYTES + EPI_WARPS * STG_BYTES + NUM_BARS * 8 + 16;
+    static constexpr size_t SMEM_BYTES = 1024 + (size_t)STAGES * STAGE_BYTES +
+                                         EPI_WARPS * (STG_BYTES + TAB_BYTES) + NUM_BARS * 8 + 16;
+    static_assert(MODE != FF_I8 || W == 1, "the tables need the room of a slot");
     static_assert(SMEM_BYTES <= 232448, "shared memory budget");
 };
 
-template <int MODE, int ACT, typename OutT>
-__global__ void __launch_bounds__(FfCfg::THREADS, 1)
+template <int MODE, int ACT, typename OutT, int W>
+__global__ void __launch_bounds__(FfCfg<MODE, W>::THREADS, 1)
     ff_tc_kernel(const __grid_constant__ FfMaps maps, const __grid_constant__ FfParams p) {
-    using Cfg = FfCfg;
+    using Cfg = FfCfg<MODE, W>;
     constexpr int STAGES = Cfg::STAGES;
     constexpr int KB = MODE == FF_I8 ? 128 : 64;  // elements of a k-block
     extern __shared__ __align__(1024) uint8_t smem_raw[];
     uint8_t* smem =
         reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     uint8_t* sA = smem;
-    uint8_t* sB = sA + STAGES * Cfg::OP_BYTES;
-    uint8_t* sStg = sB + STAGES * Cfg::OP_BYTES;
-    uint64_t* bars = reinterpret_cast<uint64_t*>(sStg + Cfg::EPI_WARPS * Cfg::STG_BYTES);
+    uint8_t* sB = sA + STAGES * Cfg::A_BYTES;
+    uint8_t* sStg = sB + STAGES * Cfg::B_BYTES;
+    float* sTab = reinterpret_cast<float*>(sStg + Cfg::EPI_WARPS * Cfg::STG_BYTES);
+    uint64_t* bars = reinterpret_cast<uint64_t*>(sStg + Cfg::EPI_WARPS * (Cfg::STG_BYTES + Cfg::TAB_BYTES));
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + Cfg::NUM_BARS);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
     volatile uint32_t* issued_slot = tmem_slot + 2;  // the odd CTA's k-block count
@@ -196,39 +211,49 @@ __global__ void __launch_bounds__(FfCfg::THREADS, 1)
             FfItem it;
             for (int idx = 0; ok && ff_item<MODE>(p, unit, units, idx, it); ++idx) {
                 const int row = it.mb * 256 + (int)rank * 128;
-                // First column of this CTA's share of B.
-                const int col = MODE == FF_GLU ? it.nb * 128 : it.nb * 256 + (int)rank * 128;
+                // First column of this CTA's share of B, and from one MMA's
+                // columns to the next one's.
+                const int col = MODE == FF_GLU ? it.nb * 128 * W : it.nb * 256 * W + (int)rank * 128;
+                constexpr int next = MODE == FF_GLU ? 128 : 256;
                 for (int kb = 0; kb < it.kbs; ++kb) {
                     if (!mbar_wait(empty0 + 8u * stage, phase ^ 1u, abort_flag)) {
                         ok = false;
                         break;
                     }
                     const uint32_t fb = mapa_shared(full0 + 8u * stage, 0);
-                    const uint32_t a = smem_u32(sA + stage * Cfg::OP_BYTES), b = smem_u32(sB + stage * Cfg::OP_BYTES);
+                    const uint32_t a = smem_u32(sA + stage * Cfg::A_BYTES), b = smem_u32(sB + stage * Cfg::B_BYTES);
                     // Both CTAs' loads complete on the even CTA's barrier.
                     if (leader) mbar_arrive_expect_tx(full0 + 8u * stage, 2 * Cfg::STAGE_BYTES);
                     const int k = kb * KB;
                     if constexpr (MODE == FF_GLU) {
                         const CUtensorMap* w = &maps.m[leader ? MG_WG : MG_WU];
                         tma_load_3d_pair(a, &maps.m[MG_X], fb, k, row, 0);
-                        tma_load_3d_pair(b, w, fb, col, k, 0);
-                        tma_load_3d_pair(b + 8192, w, fb, col + 64, k, 0);
+#pragma unroll
+                        for (int h = 0; h < 2 * W; ++h) tma_load_3d_pair(b + h * 8192, w, fb, col + 64 * h, k, 0);
                     } else if constexpr (MODE == FF_I8) {
                         tma_load_3d_pair(a, &maps.m[MI_A], fb, k, row, 0);
-                        tma_load_3d_pair(b, &maps.m[MI_B], fb, k, col, 0);
+#pragma unroll
+                        for (int h = 0; h < W; ++h)
+                            tma_load_3d_pair(b + h * Cfg::OP_BYTES, &maps.m[MI_B], fb, k, col + next * h, 0);
                     } else if (it.kind == 0) {
                         const bool up = kb >= p.half_kbs;
                         const int kk = up ? k - p.half_kbs * KB : k;
                         tma_load_3d_pair(a, &maps.m[up ? MB_DUK : MB_DGK], fb, kk, row, 0);
-                        tma_load_3d_pair(b, &maps.m[up ? MB_WUK : MB_WGK], fb, kk, col, 0);
+#pragma unroll
+                        for (int h = 0; h < W; ++h)
+                            tma_load_3d_pair(b + h * Cfg::OP_BYTES, &maps.m[up ? MB_WUK : MB_WGK], fb, kk,
+                                             col + next * h, 0);
                     } else {
                         const bool up = it.nb >= p.wt_n;
                         const CUtensorMap* v = &maps.m[up ? MB_DUN : MB_DGN];
-                        const int c = up ? col - p.wt_n * 256 : col;
+                        const int c = up ? col - p.wt_n * 256 * W : col;
                         tma_load_3d_pair(a, &maps.m[MB_XN], fb, row, k, 0);
                         tma_load_3d_pair(a + 8192, &maps.m[MB_XN], fb, row + 64, k, 0);
-                        tma_load_3d_pair(b, v, fb, c, k, 0);
-                        tma_load_3d_pair(b + 8192, v, fb, c + 64, k, 0);
+#pragma unroll
+                        for (int h = 0; h < W; ++h) {
+                            tma_load_3d_pair(b + h * Cfg::OP_BYTES, v, fb, c + next * h, k, 0);
+                            tma_load_3d_pair(b + h * Cfg::OP_BYTES + 8192, v, fb, c + next * h + 64, k, 0);
+                        }
                     }
                     ++total;
                     if (++stage == STAGES) {
@@ -283,22 +308,26 @@ __global__ void __launch_bounds__(FfCfg::THREADS, 1)
                 // Releases come from both CTAs' epilogues.
                 if (!mbar_wait<true>(tempty0 + 8u * acc, acc_phase ^ 1u, abort_flag)) break;
                 tc_fence_after();
-                const uint32_t d = tmem_base + (uint32_t)(acc * 256);
+                const uint32_t d = tmem_base + (uint32_t)(acc * 256 * W);
                 for (int kb = 0; kb < it.kbs; ++kb) {
                     if (!mbar_wait(full0 + 8u * stage, phase, abort_flag)) {
                         ok = false;
                         break;
                     }
                     tc_fence_after();
-                    uint64_t ad = a0 + (uint64_t)((stage * Cfg::OP_BYTES) >> 4);
-                    uint64_t bd = b0 + (uint64_t)((stage * Cfg::OP_BYTES) >> 4);
+                    uint64_t ad = a0 + (uint64_t)((stage * Cfg::A_BYTES) >> 4);
+                    uint64_t bd = b0 + (uint64_t)((stage * Cfg::B_BYTES) >> 4);
 #pragma unroll
                     for (int kk = 0; kk < 4; ++kk) {
                         const uint32_t more = (kb | kk) != 0 ? 1u : 0u;
-                        if constexpr (MODE == FF_I8)
-                            tc_mma_i8_pair(d, ad, bd, id, more);
-                        else
-                            tc_mma_f16_pair(d, ad, bd, id, more);
+#pragma unroll
+                        for (int h = 0; h < W; ++h) {
+                            const uint64_t bh = bd + (uint64_t)(h * (Cfg::OP_BYTES >> 4));
+                            if constexpr (MODE == FF_I8)
+                                tc_mma_i8_pair(d + 256u * h, ad, bh, id, more);
+                            else
+                                tc_mma_f16_pair(d + 256u * h, ad, bh, id, more);
+                        }
                         ad += a_step;
                         bd += b_step;
                     }
@@ -312,7 +341,7 @@ __global__ void __launch_bounds__(FfCfg::THREADS, 1)
                 if (!ok) break;
                 tc_commit_pair(mapa_shared(tfull0 + 8u * acc, 0));
                 tc_commit_pair(mapa_shared(tfull0 + 8u * acc, 1));
-                if (++acc == 2) {
+                if (++acc == Cfg::ACCS) {
                     acc = 0;
                     acc_phase ^= 1u;
                 }
@@ -357,11 +386,24 @@ __global__ void __launch_bounds__(FfCfg::THREADS, 1)
         FfItem it;
         for (int idx = 0; ff_item<MODE>(p, unit, units, idx, it); ++idx) {
             const int row0 = it.mb * 256 + (int)rank * 128 + q * 32;
+            float* tab = sTab + (warp - 2) * 256;  // this warp's 128 scales, then its 128 bias values
+            float sa = 0.f;
+            if constexpr (MODE == FF_I8) {
+                if (row0 + lane < p.M) sa = __ldg(p.sa + row0 + lane);
+                const int c0 = it.nb * 256 + wh * 128 + lane;
+#pragma unroll
+                for (int i = 0; i < 128; i += 32) {
+                    const int c = c0 + i;
+                    tab[lane + i] = c < p.N ? __ldg(p.sb + c) : 0.f;
+                    tab[128 + lane + i] = p.bias && c < p.N ? __half2float(p.bias[c]) : 0.f;
+                }
+                __syncwarp();
+            }
             bool ok = mbar_wait(tfull0 + 8u * acc, acc_phase, abort_flag);
             ok = __all_sync(0xffffffffu, ok);
             if (!ok) break;
             tc_fence_after();
-            const uint32_t t_row = tmem_base + ((uint32_t)(q * 32) << 16) + (uint32_t)(acc * 256);
+            const uint32_t t_row = tmem_base + ((uint32_t)(q * 32) << 16) + (uint32_t)(acc * 256 * W);
             auto release = [&]() {  // the accumulator is read: back to the MMA warp
                 tc_fence_before();
                 __syncwarp();
@@ -373,19 +415,21 @@ __global__ void __launch_bounds__(FfCfg::THREADS, 1)
                 }
             };
             if constexpr (MODE == FF_GLU) {
-                // This warp's 64 columns of H: G beside U.
-                const int col = it.nb * 128 + wh * 64;
-                if (row0 >= p.M || col >= p.N) {
-                    release();
-                } else {
+                // 64 columns of H per warp and MMA: G beside U.
+                const int chunks = row0 >= p.M ? 0 : min(W, max(0, (p.N - it.nb * 128 * W - wh * 64 + 127) / 128));
+                if (chunks == 0) release();
+#pragma unroll 1
+                for (int n = 0; n < chunks; ++n) {
+                    const int col = it.nb * 128 * W + n * 128 + wh * 64;
+                    const uint32_t t_gu = t_row + (uint32_t)(n * 256 + wh * 64);
                     uint32_t wH[32], wG[32], wU[32];
 #pragma unroll
                     for (int h = 0; h < 2; ++h) {
                         float g[32], u[32];
-                        tmem_ld_32x32b_x32(t_row + (uint32_t)(wh * 64 + 32 * h), g);
-                        tmem_ld_32x32b_x32(t_row + (uint32_t)(128 + wh * 64 + 32 * h), u);
+                        tmem_ld_32x32b_x32(t_gu + (uint32_t)(32 * h), g);
+                        tmem_ld_32x32b_x32(t_gu + (uint32_t)(128 + 32 * h), u);
                         tmem_wait_ld();
-                        if (h == 1) release();
+                        if (h == 1 && n == chunks - 1) release();
 #pragma unroll
                         for (int i = 0; i < 16; ++i) {
                             wG[16 * h + i] = pack_half2(g[2 * i], g[2 * i + 1]);
@@ -401,41 +445,30 @@ __global__ void __launch_bounds__(FfCfg::THREADS, 1)
                     }
                 }
             } else {
-                // 128 columns per warp, in chunks of one 128-byte row a lane.
+                // 128 W columns per warp, in chunks of one 128-byte row a lane.
                 const bool f16 = sizeof(OutT) == 2 || (MODE == FF_BACK && it.kind == 0);
                 const bool up = MODE == FF_BACK && it.kind == 1 && it.nb >= p.wt_n;
                 const int rows = MODE == FF_BACK ? (it.kind == 0 ? p.M : p.D) : p.M;
                 const int cols = MODE == FF_BACK ? (it.kind == 0 ? p.D : p.F) : p.N;
-                const int tcol = (up ? it.nb - p.wt_n : it.nb) * 256 + wh * 128;
-                const int valid = row0 < rows ? min(128, cols - tcol) : 0;
+                const int tcol = (up ? it.nb - p.wt_n : it.nb) * 256 * W + wh * 128 * W;
+                const int valid = row0 < rows ? min(128 * W, cols - tcol) : 0;
                 const int nsub = valid > 0 ? (valid + 31) / 32 : 0;  // 32-column parts that hold anything
                 const CUtensorMap* m = MODE == FF_I8 ? &maps.m[MI_C]
                                                      : &maps.m[it.kind == 0 ? MB_DX : up ? MB_DWU : MB_DWG];
                 const bool add = MODE == FF_BACK && it.kind == 1 && p.accumulate;
-                const int row = row0 + lane;
-                float sa = 0.f;
-                if constexpr (MODE == FF_I8) sa = row < p.M ? __ldg(p.sa + row) : 0.f;
                 if (nsub == 0) release();
                 uint32_t w[32];
 #pragma unroll 1
                 for (int s = 0; s < nsub; ++s) {
                     float v[32];
-                    tmem_ld_32x32b_x32(t_row + (uint32_t)(wh * 128 + 32 * s), v);
+                    tmem_ld_32x32b_x32(t_row + (uint32_t)(wh * 128 * W + 32 * s), v);
                     tmem_wait_ld();
                     if (s == nsub - 1) release();
                     const int col = tcol + 32 * s;
                     if constexpr (MODE == FF_I8) {
-                        const bool inside = col + 32 <= p.N;
 #pragma unroll
                         for (int i = 0; i < 32; i += 4) {
-                            float4 c;
-                            if (inside && p.sb_vec) {
-                                c = __ldg(reinterpret_cast<const float4*>(p.sb + col + i));
-                            } else {
-                                const int e = p.N - 1;
-                                c = make_float4(__ldg(p.sb + min(col + i, e)), __ldg(p.sb + min(col + i + 1, e)),
-                                                __ldg(p.sb + min(col + i + 2, e)), __ldg(p.sb + min(col + i + 3, e)));
-                            }
+                            const float4 c = *reinterpret_cast<const float4*>(tab + 32 * s + i);
                             v[i] = (float)__float_as_int(v[i]) * sa * c.x;
                             v[i + 1] = (float)__float_as_int(v[i + 1]) * sa * c.y;
                             v[i + 2] = (float)__float_as_int(v[i + 2]) * sa * c.z;
@@ -443,17 +476,12 @@ __global__ void __launch_bounds__(FfCfg::THREADS, 1)
                         }
                         if (p.bias) {
 #pragma unroll
-                            for (int i = 0; i < 32; i += 8) {
-                                float b[8];
-                                if (inside && p.bias_vec) {
-                                    unpack_h8(__ldg(reinterpret_cast<const uint4*>(p.bias + col + i)), b);
-                                } else {
-#pragma unroll
-                                    for (int e = 0; e < 8; ++e)
-                                        b[e] = __half2float(p.bias[min(col + i + e, p.N - 1)]);
-                                }
-#pragma unroll
-                                for (int e = 0; e < 8; ++e) v[i + e] += b[e];
+                            for (int i = 0; i < 32; i += 4) {
+                                const float4 b = *reinterpret_cast<const float4*>(tab + 128 + 32 * s + i);
+                                v[i] += b.x;
+                                v[i + 1] += b.y;
+                                v[i + 2] += b.z;
+                                v[i + 3] += b.w;
                             }
                         }
                     }
@@ -477,23 +505,35 @@ __global__ void __launch_bounds__(FfCfg::THREADS, 1)
                         store(m, w, ccol, row0, add);
                     } else {
                         // Rows of C that are not 16-byte aligned: the staged
-                        // rows go out one after another, a warp per row.
+                        // rows go out one after another, a warp per row, eight
+                        // rows in flight.
                         stage_rows(w);
                         __syncwarp();
-                        const int n = f16 ? 64 : 32, left = min(n, p.N - ccol), last = min(32, p.M - row0);
-                        for (int r = 0; r < last; ++r) {
-                            OutT* c = static_cast<OutT*>(p.C) + (long long)(row0 + r) * p.ldc + ccol;
-                            for (int e = lane; e < left; e += 32) {
-                                const int byte = e * (int)sizeof(OutT);
-                                c[e] = *reinterpret_cast<const OutT*>(sbuf + r * 128 + (((byte >> 4) ^ (r & 7)) << 4) +
-                                                                      (byte & 15));
+                        constexpr int n = 128 / (int)sizeof(OutT);
+                        const int left = p.N - ccol, last = min(32, p.M - row0);
+#pragma unroll
+                        for (int e0 = 0; e0 < n; e0 += 32) {
+                            const int byte = (e0 + lane) * (int)sizeof(OutT);
+                            const uint8_t* from = sbuf + (byte & 15);
+                            OutT* to = static_cast<OutT*>(p.C) + (long long)row0 * p.ldc + ccol + e0 + lane;
+                            if (e0 + lane >= left) continue;
+#pragma unroll 1
+                            for (int r = 0; r < last; r += 8) {
+                                OutT x[8];
+#pragma unroll
+                                for (int i = 0; i < 8; ++i)
+                                    x[i] = *reinterpret_cast<const OutT*>(from + (r + i) * 128 + (((byte >> 4) ^ i) << 4));
+#pragma unroll
+                                for (int i = 0; i < 8; ++i)
+                                    if (r + i < last) to[(long long)(r + i) * p.ldc] = x[i];
                             }
                         }
                         __syncwarp();
                     }
                 }
             }
-            if (++acc == 2) {
+            if constexpr (MODE == FF_I8) __syncwarp();  // the table is read
+            if (++acc == Cfg::ACCS) {
                 acc = 0;
                 acc_phase ^= 1u;
             }
@@ -533,13 +573,13 @@ inline bool ff_map(CUtensorMap* m, const void* base, CUtensorMapDataType dt, int
 // CTA pairs of the kernel that device `dev` holds at once (SMs pair up
 // within a GPC, so this can be below SMs / 2).  Also sets the kernel's
 // shared-memory limit there; asked once per device and kernel.
-template <int MODE, int ACT, typename OutT>
+template <int MODE, int ACT, typename OutT, int W>
 inline int ff_units(int dev) {
     static int cache[64] = {0};
     int& v = cache[dev & 63];
     if (v == 0) {
-        auto kern = ff_tc_kernel<MODE, ACT, OutT>;
-        if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)FfCfg::SMEM_BYTES) !=
+        auto kern = ff_tc_kernel<MODE, ACT, OutT, W>;
+        if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)FfCfg<MODE, W>::SMEM_BYTES) !=
             cudaSuccess)
             return 0;
         const int sms = device_sm_count(dev);
@@ -549,8 +589,8 @@ inline int ff_units(int dev) {
         attr[0].val.clusterDim.x = 2;
         attr[0].val.clusterDim.y = 1;
         attr[0].val.clusterDim.z = 1;
-        cfg.blockDim = dim3(FfCfg::THREADS);
-        cfg.dynamicSmemBytes = FfCfg::SMEM_BYTES;
+        cfg.blockDim = dim3(FfCfg<MODE, W>::THREADS);
+        cfg.dynamicSmemBytes = FfCfg<MODE, W>::SMEM_BYTES;
         cfg.attrs = attr;
         cfg.numAttrs = 1;
         cfg.gridDim = dim3(sms & ~1);
@@ -564,7 +604,7 @@ inline int ff_units(int dev) {
     return v;
 }
 
-template <int MODE, int ACT, typename OutT>
+template <int MODE, int ACT, typename OutT, int W>
 inline pax_status_t ff_launch(const FfMaps& maps, const FfParams& p, int units, cudaStream_t stream) {
     cudaLaunchConfig_t cfg = {};
     cudaLaunchAttribute attr[2];
@@ -575,12 +615,12 @@ inline pax_status_t ff_launch(const FfMaps& maps, const FfParams& p, int units, 
     attr[1].val.clusterDim.y = 1;
     attr[1].val.clusterDim.z = 1;
     cfg.gridDim = dim3(2 * units);
-    cfg.blockDim = dim3(FfCfg::THREADS);
-    cfg.dynamicSmemBytes = FfCfg::SMEM_BYTES;
+    cfg.blockDim = dim3(FfCfg<MODE, W>::THREADS);
+    cfg.dynamicSmemBytes = FfCfg<MODE, W>::SMEM_BYTES;
     cfg.stream = stream;
     cfg.attrs = attr;
     cfg.numAttrs = 2;
-    return cudaLaunchKernelEx(&cfg, ff_tc_kernel<MODE, ACT, OutT>, maps, p) == cudaSuccess ? PAX_OK : PAX_ERR_CUDA;
+    return cudaLaunchKernelEx(&cfg, ff_tc_kernel<MODE, ACT, OutT, W>, maps, p) == cudaSuccess ? PAX_OK : PAX_ERR_CUDA;
 }
 
 }  // namespace pax
