@@ -179,11 +179,29 @@ pax_status_t pax_glu_backward_ex(const pax_glu_grad_desc_t* desc, cudaStream_t s
     if ((st = device_ok("pax_glu_backward_ex")) != PAX_OK) return st;
     st = glu_grad_rows(p, stream);
     if (st == PAX_OK && (p.dX || p.dWg)) {
-        if (glu_back_tc_ok(p)) {
-            st = glu_back_tc(p, stream);
-        } else {
-            if (p.dX) st = glu_dx_any(p, stream);
-            if (st == PAX_OK && p.dWg) st = glu_dw_any(p, stream);
+        // Few tokens leave dX too few tiles of too many k-blocks for one
+        // launch with the weight gradients: it then runs apart, split along F.
+        // The second launch counts as 6 k-blocks, about 2 us.  The choice
+        // goes by the shape, not by which gradients are asked for, so that
+        // dX has the same bits either way.
+        GluGradProblem rest = p;
+        if (glu_dx_skinny_ok(p)) {
+            GluGradProblem x = p, w = p, both = p;
+            x.dWg = x.dWu = nullptr;
+            w.dX = nullptr;
+            w.dWg = w.dWu = both.dWg = both.dWu = p.dX;  // asked for; not read here
+            if (!glu_back_tc_ok(x) || glu_dx_skinny_time(p) + glu_back_tc_time(w) + 6.0 < glu_back_tc_time(both)) {
+                st = glu_dx_skinny(p, stream);
+                rest.dX = nullptr;
+            }
+        }
+        if (st == PAX_OK && (rest.dX || rest.dWg)) {
+            if (glu_back_tc_ok(rest)) {
+                st = glu_back_tc(rest, stream);
+            } else {
+                if (rest.dX) st = glu_dx_any(rest, stream);
+                if (st == PAX_OK && rest.dWg) st = glu_dw_any(rest, stream);
+            }
         }
     }
     return done(st, "pax_glu_backward_ex");

@@ -47,13 +47,20 @@ pax_status_t gemm_i8_any(const I8Problem& p, cudaStream_t stream);
 bool glu_tc_ok(const GluProblem& p);
 pax_status_t glu_tc(const GluProblem& p, cudaStream_t stream);
 bool glu_back_tc_ok(const GluGradProblem& p);
+double glu_back_tc_time(const GluGradProblem& p);
 pax_status_t glu_back_tc(const GluGradProblem& p, cudaStream_t stream);
 bool gemm_i8_tc_ok(const I8Problem& p);
 pax_status_t gemm_i8_tc(const I8Problem& p, cudaStream_t stream);
 int read_clear_device_error_ff_tc();
 bool set_wait_limit_ff_tc(unsigned long long ns);
 
-// feed_forward_skinny.cu: at most 64 tokens.
+// feed_forward_skinny.cu: the gated and the 8-bit product of at most 64
+// tokens; the input gradient of any number, with its modelled time in
+// k-blocks (about 0.36 us each), as glu_back_tc_time's for the tiles of
+// glu_back_tc.
+bool glu_dx_skinny_ok(const GluGradProblem& p);
+double glu_dx_skinny_time(const GluGradProblem& p);
+pax_status_t glu_dx_skinny(const GluGradProblem& p, cudaStream_t stream);
 bool glu_skinny_ok(const GluProblem& p);
 pax_status_t glu_skinny(const GluProblem& p, cudaStream_t stream);
 bool gemm_i8_skinny_ok(const I8Problem& p);

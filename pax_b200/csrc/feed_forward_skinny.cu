@@ -1,12 +1,15 @@
-// feed_forward_skinny.cu -- the gated and the 8-bit product for few tokens
-// (decoding), on tcgen05.
+// feed_forward_skinny.cu -- the gated and the 8-bit product and the input
+// gradient for few tokens (decoding, short sequences), on tcgen05.
 //
-// With few tokens both products are bound by reading the weights once.  The
+// With few tokens these products are bound by reading the weights once.  The
 // operands are swapped: 128 weight columns are the 128 rows of the MMA and
 // the tokens, padded to MP = 16, 32, 48 or 64, its columns, so that no
 // tensor work is spent on absent tokens:
-//   gated   64 columns of Wg and the same 64 of Wu (MN-major, as they lie)
-//   8-bit   128 rows of B (K-major, as they lie)
+//   gated       64 columns of Wg and the same 64 of Wu (MN-major, as they lie)
+//   8-bit       128 rows of B (K-major, as they lie)
+//   input grad  128 rows of Wg, then of Wu, along F (K-major, as they lie)
+// More than 64 tokens run as equal chunks (blockIdx.y), each reading the
+// weights again, mostly from L2.
 //
 // A tile of weight columns is too coarse a unit of work for 148 SMs, so a
 // cluster of S CTAs shares each tile along K: CTA r takes k-blocks r, r + S,
@@ -17,8 +20,8 @@
 // order, applies the epilogue and stores.  No global workspace, no atomics,
 // and the same bits every time.
 //
-// A cluster computes one tile and ends.  Two CTAs are resident per SM, so
-// that one streams while the other starts up or reduces, and the hardware
+// A cluster computes one tile and ends.  R = 2 or 3 CTAs are resident per SM,
+// so that one streams while another starts up or reduces, and the hardware
 // hands the next cluster to whichever SMs are free.
 //
 // 192 threads: warp 0 TMA producer, warp 1 MMA issuer, warps 2-5 epilogue
@@ -32,11 +35,13 @@ namespace pax {
 
 namespace {
 
-enum : int { FS_GLU = 0, FS_I8 = 1 };
+enum : int { FS_GLU = 0, FS_I8 = 1, FS_DX = 2 };
 
 struct FsParams {
     int M, N, kbs;  // tokens, weight columns, k-blocks
-    // FS_GLU
+    int rows;       // tokens of a chunk
+    int half;       // FS_DX: k-blocks of the first term
+    // FS_GLU; FS_DX: the gradient in H
     __half *H, *G, *U;
     long long ldh, ldg, ldu;
     int act;
@@ -48,13 +53,14 @@ struct FsParams {
     int c_f16;
 };
 
-template <int MODE, int MP>
+template <int MODE, int MP, int R>
 struct FsCfg {
     static constexpr int KB = MODE == FS_I8 ? 128 : 64;    // k of a ring slot: 128 bytes
-    static constexpr int TILE = MODE == FS_I8 ? 128 : 64;  // output columns of a tile
+    static constexpr int TILE = MODE == FS_GLU ? 64 : 128;  // output columns of a tile
     static constexpr uint32_t W_BYTES = 16384, X_BYTES = MP * 128, STAGE_BYTES = W_BYTES + X_BYTES;
-    // As many slots as let two CTAs share an SM.
-    static constexpr int STAGES = (int)((113 * 1024 - 1024 - 256) / STAGE_BYTES);
+    // As many slots as let R CTAs share an SM.
+    static constexpr uint32_t SHARE = R == 2 ? 113 * 1024 : 75 * 1024;
+    static constexpr int STAGES = (int)((SHARE - 1024 - 256) / STAGE_BYTES);
     static constexpr uint32_t NUM_BARS = 2 * STAGES + 1;
     static constexpr size_t SMEM_BYTES = 1024 + (size_t)STAGES * STAGE_BYTES + NUM_BARS * 8 + 16;
     static constexpr uint32_t TMEM_COLS = MP <= 32 ? 32 : 64;
@@ -62,7 +68,7 @@ struct FsCfg {
     // columns (two values each for the gated product) for MP tokens, up to
     // 128 + 2 (S - 1) values a token.
     static_assert(MP * 144 * 4 <= STAGES * STAGE_BYTES, "the ring holds the contributions");
-    static_assert(SMEM_BYTES <= 113 * 1024 && STAGES >= 4, "shared memory of half an SM");
+    static_assert(SMEM_BYTES <= SHARE && STAGES >= 3, "an R-th of an SM's shared memory");
 };
 
 // First column of part j of a tile shared by S CTAs.
@@ -71,11 +77,12 @@ __device__ __forceinline__ int part_start(int j, int S) {
     return (j * TILE + S - 1) / S;
 }
 
-template <int MODE, int MP>
-__global__ void __launch_bounds__(192, 2)
+template <int MODE, int MP, int R>
+__global__ void __launch_bounds__(192, R)
     ff_skinny_kernel(const __grid_constant__ CUtensorMap tmW0, const __grid_constant__ CUtensorMap tmW1,
-                     const __grid_constant__ CUtensorMap tmX, const __grid_constant__ FsParams p) {
-    using Cfg = FsCfg<MODE, MP>;
+                     const __grid_constant__ CUtensorMap tmX, const __grid_constant__ CUtensorMap tmX1,
+                     const __grid_constant__ FsParams p) {
+    using Cfg = FsCfg<MODE, MP, R>;
     constexpr int STAGES = Cfg::STAGES, TILE = Cfg::TILE;
     extern __shared__ __align__(1024) uint8_t smem_raw[];
     uint8_t* smem =
@@ -93,6 +100,7 @@ __global__ void __launch_bounds__(192, 2)
     asm("mov.u32 %0, %%cluster_nctarank;" : "=r"(S));
     const int rank = (int)cluster_ctarank();
     const int tile = (int)blockIdx.x / S;
+    const int m0 = (int)blockIdx.y * p.rows, M = min(p.rows, p.M - m0);  // this chunk's tokens
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < STAGES; ++s) {
@@ -127,14 +135,17 @@ __global__ void __launch_bounds__(192, 2)
                 const uint32_t fb = full0 + 8u * stage;
                 const uint32_t w = smem_u32(smem + stage * Cfg::STAGE_BYTES);
                 const int k = kb * Cfg::KB;
-                mbar_arrive_expect_tx(fb, Cfg::STAGE_BYTES);
+                mbar_arrive_expect_tx(fb, Cfg::W_BYTES + (uint32_t)p.rows * 128u);
                 if constexpr (MODE == FS_GLU) {
                     tma_load_3d(w, &tmW0, fb, col, k, 0);
                     tma_load_3d(w + 8192, &tmW1, fb, col, k, 0);
+                    tma_load_3d(w + Cfg::W_BYTES, &tmX, fb, k, m0, 0);
                 } else {
-                    tma_load_3d(w, &tmW0, fb, k, col, 0);
+                    const bool second = MODE == FS_DX && kb >= p.half;
+                    const int kk = second ? k - p.half * Cfg::KB : k;
+                    tma_load_3d(w, second ? &tmW1 : &tmW0, fb, kk, col, 0);
+                    tma_load_3d(w + Cfg::W_BYTES, second ? &tmX1 : &tmX, fb, kk, m0, 0);
                 }
-                tma_load_3d(w + Cfg::W_BYTES, &tmX, fb, k, 0, 0);
                 ++total;
                 if (++stage == STAGES) {
                     stage = 0;
@@ -157,7 +168,7 @@ __global__ void __launch_bounds__(192, 2)
             const uint64_t w0 = MODE == FS_GLU ? umma_desc_sw128(smem_u32(smem), 8192, 1024)
                                                : umma_desc_sw128(smem_u32(smem), 16, 1024);
             const uint64_t x0 = umma_desc_sw128(smem_u32(smem) + Cfg::W_BYTES, 16, 1024);
-            const uint32_t id = MODE == FS_GLU ? umma_idesc_f16(128, MP, true, false) : umma_idesc_i8(128, MP);
+            const uint32_t id = MODE == FS_I8 ? umma_idesc_i8(128, MP) : umma_idesc_f16(128, MP, MODE == FS_GLU, false);
             for (int kb = rank; kb < p.kbs; kb += S) {
                 if (!mbar_wait(full0 + 8u * stage, phase, abort_flag)) break;
                 tc_fence_after();
@@ -166,10 +177,11 @@ __global__ void __launch_bounds__(192, 2)
                 for (int kk = 0; kk < 4; ++kk) {
                     const uint32_t more = (kb != rank || kk != 0) ? 1u : 0u;
                     const uint64_t xd = x0 + at + (uint64_t)(kk * 2);
-                    if constexpr (MODE == FS_GLU)
-                        tc_mma_f16(tmem_base, w0 + at + (uint64_t)(kk * 128), xd, id, more);
+                    const uint64_t wd = w0 + at + (uint64_t)(kk * (MODE == FS_GLU ? 128 : 2));
+                    if constexpr (MODE == FS_I8)
+                        tc_mma_i8(tmem_base, wd, xd, id, more);
                     else
-                        tc_mma_i8(tmem_base, w0 + at + (uint64_t)(kk * 2), xd, id, more);
+                        tc_mma_f16(tmem_base, wd, xd, id, more);
                 }
                 tc_commit(empty0 + 8u * stage);
                 if (++stage == STAGES) {
@@ -202,10 +214,10 @@ __global__ void __launch_bounds__(192, 2)
         const int dest = f * S / TILE;
         const int dstart = part_start<TILE>(dest, S), dwidth = part_start<TILE>(dest + 1, S) - dstart;
         const int at = f - dstart + (MODE == FS_GLU && l >= TILE ? dwidth : 0);
-        const uint32_t to = mapa_shared(smem_u32(smem) + (uint32_t)(rank * p.M * stride + at) * 4u, (uint32_t)dest);
+        const uint32_t to = mapa_shared(smem_u32(smem) + (uint32_t)(rank * M * stride + at) * 4u, (uint32_t)dest);
 #pragma unroll
         for (int m = 0; m < MP; ++m)
-            if (m < p.M) st_shared_cluster_f32(to + (uint32_t)(m * stride * 4), v[m]);
+            if (m < M) st_shared_cluster_f32(to + (uint32_t)(m * stride * 4), v[m]);
     }
     __syncwarp();
     cluster_sync();  // the contributions are in; nothing remote happens after this
@@ -216,31 +228,35 @@ __global__ void __launch_bounds__(192, 2)
     if (*abort_flag) return;
     const float* r = reinterpret_cast<const float*>(smem);
     const int pstart = part_start<TILE>(rank, S), pwidth = part_start<TILE>(rank + 1, S) - pstart;
-    for (int e = (int)threadIdx.x; e < p.M * pwidth; e += 192) {
+    for (int e = (int)threadIdx.x; e < M * pwidth; e += 192) {
         const int m = e / pwidth, c = e - m * pwidth;
-        const long long col = (long long)tile * TILE + pstart + c;
+        const long long row = m0 + m, col = (long long)tile * TILE + pstart + c;
         if (col >= p.N) continue;
         if constexpr (MODE == FS_GLU) {
             float g = 0.f, u = 0.f;
             for (int s = 0; s < S; ++s) {
-                const float* x = r + (s * p.M + m) * stride + c;
+                const float* x = r + (s * M + m) * stride + c;
                 g += x[0];
                 u += x[pwidth];
             }
-            p.H[m * p.ldh + col] = __float2half_rn(act_value_rt(p.act, g) * u);
+            p.H[row * p.ldh + col] = __float2half_rn(act_value_rt(p.act, g) * u);
             if (p.G) {
-                p.G[m * p.ldg + col] = __float2half_rn(g);
-                p.U[m * p.ldu + col] = __float2half_rn(u);
+                p.G[row * p.ldg + col] = __float2half_rn(g);
+                p.U[row * p.ldu + col] = __float2half_rn(u);
             }
+        } else if constexpr (MODE == FS_DX) {
+            float sum = 0.f;
+            for (int s = 0; s < S; ++s) sum += r[(s * M + m) * stride + c];
+            p.H[row * p.ldh + col] = __float2half_rn(sum);
         } else {
             int sum = 0;
-            for (int s = 0; s < S; ++s) sum += __float_as_int(r[(s * p.M + m) * stride + c]);
-            float o = (float)sum * p.sa[m] * p.sb[col];
+            for (int s = 0; s < S; ++s) sum += __float_as_int(r[(s * M + m) * stride + c]);
+            float o = (float)sum * p.sa[row] * p.sb[col];
             if (p.bias) o += __half2float(p.bias[col]);
             if (p.c_f16)
-                static_cast<__half*>(p.C)[m * p.ldc + col] = __float2half_rn(o);
+                static_cast<__half*>(p.C)[row * p.ldc + col] = __float2half_rn(o);
             else
-                static_cast<float*>(p.C)[m * p.ldc + col] = o;
+                static_cast<float*>(p.C)[row * p.ldc + col] = o;
         }
     }
 }
@@ -261,31 +277,49 @@ bool fs_map(CUtensorMap* m, const void* base, bool i8, long long rows, long long
 
 constexpr int kMaxSplit = 8;
 
-template <int MODE, int MP>
-bool fs_prepare(int dev) {
-    static bool done[64] = {false};
-    bool& d = done[dev & 63];
-    if (!d)
-        d = cudaFuncSetAttribute(ff_skinny_kernel<MODE, MP>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                 (int)FsCfg<MODE, MP>::SMEM_BYTES) == cudaSuccess;
-    return d;
+
+// Clusters of S CTAs that device `dev` holds at once: R times what it holds
+// with one CTA per SM, which is what the runtime answers (a cluster's CTAs
+// share a GPC, so this can be below the SMs' room).  Also sets the kernel's
+// shared-memory limit there.  Asked once per device, kernel and S; 0: error.
+template <int MODE, int MP, int R>
+int fs_clusters(int dev, int S) {
+    static int cache[64][kMaxSplit + 1] = {{0}};
+    int& v = cache[dev & 63][S];
+    if (v == 0) {
+        using Cfg = FsCfg<MODE, MP, R>;
+        auto kern = ff_skinny_kernel<MODE, MP, R>;
+        if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)Cfg::SMEM_BYTES) !=
+            cudaSuccess)
+            return 0;
+        cudaLaunchConfig_t cfg = {};
+        cudaLaunchAttribute attr[1];
+        attr[0].id = cudaLaunchAttributeClusterDimension;
+        attr[0].val.clusterDim.x = S;
+        attr[0].val.clusterDim.y = 1;
+        attr[0].val.clusterDim.z = 1;
+        cfg.blockDim = dim3(192);
+        cfg.dynamicSmemBytes = Cfg::SMEM_BYTES;
+        cfg.attrs = attr;
+        cfg.numAttrs = 1;
+        cfg.gridDim = dim3((unsigned)(4 * device_sm_count(dev) * S));  // the answer is capped by the grid
+        int n = 0;
+        if (cudaOccupancyMaxActiveClusters(&n, kern, &cfg) != cudaSuccess) {
+            cudaGetLastError();
+            return 0;
+        }
+        v = R * n;
+    }
+    return v;
 }
 
-template <int MODE, int MP>
-pax_status_t launch_skinny(const CUtensorMap& w0, const CUtensorMap& w1, const CUtensorMap& x, const FsParams& p,
-                           cudaStream_t stream) {
-    using Cfg = FsCfg<MODE, MP>;
-    const int dev = current_device(), sms = device_sm_count(dev);
-    if (!fs_prepare<MODE, MP>(dev)) return PAX_ERR_CUDA;
-    const long long tiles = (p.N + Cfg::TILE - 1) / Cfg::TILE;
-    // As many CTAs as are resident at once, with at least four k-blocks each.
-    // A CTA that has to wait for another's end costs more than the finer
-    // split gains: 1x2048x5504 in 86 / 172 / 258 / 344 CTAs takes 15.4 / 13.5
-    // / 13.6 / 17.7 us, 24x4096x11264 in 176 / 352 / 704 takes 35.6 / 42.9 /
-    // 45.0.
-    int S = 1;
-    while (S < kMaxSplit && tiles * (S + 1) <= 2 * sms && p.kbs >= 4 * (S + 1)) ++S;
-    if (tiles * S > 0x7fffffffLL) return PAX_ERR_UNSUPPORTED;
+struct FsMaps {
+    CUtensorMap w0, w1, x0, x1;
+};
+
+template <int MODE, int MP, int R>
+pax_status_t launch_split(const FsMaps& m, const FsParams& p, long long tiles, int S, cudaStream_t stream) {
+    using Cfg = FsCfg<MODE, MP, R>;
     cudaLaunchConfig_t cfg = {};
     cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -294,29 +328,96 @@ pax_status_t launch_skinny(const CUtensorMap& w0, const CUtensorMap& w1, const C
     attr[1].val.clusterDim.x = S;
     attr[1].val.clusterDim.y = 1;
     attr[1].val.clusterDim.z = 1;
-    cfg.gridDim = dim3((unsigned)(tiles * S));
+    cfg.gridDim = dim3((unsigned)(tiles * S), (unsigned)((p.M + p.rows - 1) / p.rows));
     cfg.blockDim = dim3(192);
     cfg.dynamicSmemBytes = Cfg::SMEM_BYTES;
     cfg.stream = stream;
     cfg.attrs = attr;
     cfg.numAttrs = 2;
-    return cudaLaunchKernelEx(&cfg, ff_skinny_kernel<MODE, MP>, w0, w1, x, p) == cudaSuccess ? PAX_OK : PAX_ERR_CUDA;
+    return cudaLaunchKernelEx(&cfg, ff_skinny_kernel<MODE, MP, R>, m.w0, m.w1, m.x0, m.x1, p) == cudaSuccess
+               ? PAX_OK
+               : PAX_ERR_CUDA;
+}
+
+// Time of n resident CTAs of kb k-blocks each, in k-blocks at an SM's share of
+// the memory bandwidth (44 GB/s).  SMs share the bandwidth evenly; a CTA
+// alone takes in at most about one share with R = 2 (0.85 with R = 3, whose
+// ring is shorter).  So first all SMs work off the CTAs that each of them
+// has, then those with one more CTA finish, faster the fewer they are.
+// Measured against it at D = 4096, with a fixed 2 us on top: 74 tiles unsplit,
+// R = 2, 22.0 us (model 23); 176 tiles, R = 2, 35.0 (35), in pairs at R = 3,
+// 31.0 (28); 350 tiles, R = 3, 57.9 (55).  Over 19 shapes of 1 to 64 tokens
+// the choice is the best of 14 tried by hand, or within 5 % of it.
+double fs_wave_time(long long n, double kb, int R, int sms) {
+    const double cap = R == 2 ? 1.0 : 0.85;
+    const long long a = n / sms, rem = n % sms;
+    const double t = a > 0 ? a * kb / (a * cap < 1 ? a * cap : 1) : 0;
+    if (rem == 0) return t;
+    const double own = (a + 1) * cap, share = (double)sms / rem;
+    return t + ((a + 1) * kb - t * (own < 1 ? own : 1)) / (own < share ? own : share);
+}
+
+// The split of a problem and its modelled time in k-blocks.
+struct FsPlan {
+    int S = 1, R = 2;
+    double time = -1;
+};
+
+template <int MODE, int MP>
+FsPlan fs_plan(const FsParams& p) {
+    const int dev = current_device(), sms = device_sm_count(dev);
+    constexpr int TILE = FsCfg<MODE, MP, 2>::TILE;
+    const long long tiles = (long long)((p.N + TILE - 1) / TILE) * ((p.M + p.rows - 1) / p.rows);
+    FsPlan best;
+    // The residency and split with the shortest modelled time, among those
+    // whose clusters are all resident at once (1x2048x5504 in fives at three
+    // per SM, of which 78 of 86 clusters are resident: 15.7 us, in threes at
+    // two per SM 10.8); or unsplit in several waves.
+    for (int r = 2; r <= 3; ++r)
+        for (int s = 1; s <= kMaxSplit; ++s) {
+            if (s > 1 && (tiles * s > (long long)r * sms || p.kbs < 2 * s)) break;
+            const long long n = r == 2 ? fs_clusters<MODE, MP, 2>(dev, s) : fs_clusters<MODE, MP, 3>(dev, s);
+            if (n <= 0 || (s > 1 && tiles > n)) continue;
+            const long long waves = (tiles - 1) / n;  // before the last one
+            const double kb = (p.kbs + s - 1) / s;
+            const double t = (double)waves * r * kb + fs_wave_time((tiles - waves * n) * s, kb, r, sms) + (s > 1 ? 1 : 0);
+            if (best.time < 0 || t < best.time || (t == best.time && r == best.R)) {
+                best.time = t;
+                best.S = s;
+                best.R = r;
+            }
+        }
+    return best;
+}
+
+template <int MODE, int MP>
+pax_status_t launch_skinny(const FsMaps& m, const FsParams& p, cudaStream_t stream) {
+    const FsPlan plan = fs_plan<MODE, MP>(p);
+    if (plan.time < 0) return PAX_ERR_CUDA;
+    constexpr int TILE = FsCfg<MODE, MP, 2>::TILE;
+    const long long tiles = (p.N + TILE - 1) / TILE;
+    if (tiles * plan.S > 0x7fffffffLL) return PAX_ERR_UNSUPPORTED;
+    return plan.R == 2 ? launch_split<MODE, MP, 2>(m, p, tiles, plan.S, stream)
+                       : launch_split<MODE, MP, 3>(m, p, tiles, plan.S, stream);
 }
 
 template <int MODE>
-pax_status_t launch_tokens(const CUtensorMap& w0, const CUtensorMap& w1, const CUtensorMap& x, const FsParams& p,
-                           cudaStream_t stream) {
-    if (p.M <= 16) return launch_skinny<MODE, 16>(w0, w1, x, p, stream);
-    if (p.M <= 32) return launch_skinny<MODE, 32>(w0, w1, x, p, stream);
-    if (p.M <= 48) return launch_skinny<MODE, 48>(w0, w1, x, p, stream);
-    return launch_skinny<MODE, 64>(w0, w1, x, p, stream);
+pax_status_t launch_tokens(const FsMaps& m, const FsParams& p, cudaStream_t stream) {
+    if (p.rows <= 16) return launch_skinny<MODE, 16>(m, p, stream);
+    if (p.rows <= 32) return launch_skinny<MODE, 32>(m, p, stream);
+    if (p.rows <= 48) return launch_skinny<MODE, 48>(m, p, stream);
+    return launch_skinny<MODE, 64>(m, p, stream);
+}
+
+// Equal chunks of at most 64 tokens.
+int chunk_rows(long long M) {
+    const long long chunks = (M + 63) / 64;
+    return (int)((M + chunks - 1) / chunks);
 }
 
 bool rows16(const void* p, long long ld, int elem) {
     return (reinterpret_cast<uintptr_t>(p) & 15u) == 0 && (ld * elem) % 16 == 0;
 }
-
-uint32_t padded(long long M) { return (uint32_t)((M + 15) / 16 * 16); }
 
 }  // namespace
 
@@ -325,18 +426,56 @@ bool glu_skinny_ok(const GluProblem& q) {
 }
 
 pax_status_t glu_skinny(const GluProblem& q, cudaStream_t stream) {
-    CUtensorMap wg, wu, x;
-    if (!fs_map(&wg, q.Wg, false, q.D, q.F, q.ldwg, 64, 64) || !fs_map(&wu, q.Wu, false, q.D, q.F, q.ldwu, 64, 64) ||
-        !fs_map(&x, q.X, false, q.M, q.D, q.ldx, 64, padded(q.M)))
-        return PAX_ERR_CUDA;
+    FsMaps m;
     FsParams p = {};
     p.M = (int)q.M;
     p.N = (int)q.F;
     p.kbs = (int)((q.D + 63) / 64);
+    p.rows = chunk_rows(q.M);
+    if (!fs_map(&m.w0, q.Wg, false, q.D, q.F, q.ldwg, 64, 64) || !fs_map(&m.w1, q.Wu, false, q.D, q.F, q.ldwu, 64, 64) ||
+        !fs_map(&m.x0, q.X, false, q.M, q.D, q.ldx, 64, (uint32_t)p.rows))
+        return PAX_ERR_CUDA;
+    m.x1 = m.x0;
     p.H = q.H, p.G = q.G, p.U = q.U;
     p.ldh = q.ldh, p.ldg = q.ldg, p.ldu = q.ldu;
     p.act = q.act;
-    return launch_tokens<FS_GLU>(wg, wu, x, p, stream);
+    return launch_tokens<FS_GLU>(m, p, stream);
+}
+
+bool glu_dx_skinny_ok(const GluGradProblem& q) {
+    return q.dX && q.M > 0 && q.M <= 64LL * 65535 && q.D > 0 && q.F > 0 && rows16(q.dG, q.lddg, 2) &&
+           rows16(q.dU, q.lddu, 2) && rows16(q.Wg, q.ldwg, 2) && rows16(q.Wu, q.ldwu, 2);
+}
+
+static void dx_params(const GluGradProblem& q, FsParams& p) {
+    p.M = (int)q.M;
+    p.N = (int)q.D;
+    p.half = (int)((q.F + 63) / 64);
+    p.kbs = 2 * p.half;
+    p.rows = chunk_rows(q.M);
+    p.H = q.dX;
+    p.ldh = q.lddx;
+}
+
+double glu_dx_skinny_time(const GluGradProblem& q) {
+    FsParams p = {};
+    dx_params(q, p);
+    const double t = p.rows <= 16   ? fs_plan<FS_DX, 16>(p).time
+                     : p.rows <= 32 ? fs_plan<FS_DX, 32>(p).time
+                     : p.rows <= 48 ? fs_plan<FS_DX, 48>(p).time
+                                    : fs_plan<FS_DX, 64>(p).time;
+    return t < 0 ? 1e30 : t;
+}
+
+pax_status_t glu_dx_skinny(const GluGradProblem& q, cudaStream_t stream) {
+    FsMaps m;
+    FsParams p = {};
+    dx_params(q, p);
+    if (!fs_map(&m.w0, q.Wg, false, q.D, q.F, q.ldwg, 64, 128) || !fs_map(&m.w1, q.Wu, false, q.D, q.F, q.ldwu, 64, 128) ||
+        !fs_map(&m.x0, q.dG, false, q.M, q.F, q.lddg, 64, (uint32_t)p.rows) ||
+        !fs_map(&m.x1, q.dU, false, q.M, q.F, q.lddu, 64, (uint32_t)p.rows))
+        return PAX_ERR_CUDA;
+    return launch_tokens<FS_DX>(m, p, stream);
 }
 
 bool gemm_i8_skinny_ok(const I8Problem& q) {
@@ -344,18 +483,22 @@ bool gemm_i8_skinny_ok(const I8Problem& q) {
 }
 
 pax_status_t gemm_i8_skinny(const I8Problem& q, cudaStream_t stream) {
-    CUtensorMap w, x;
-    if (!fs_map(&w, q.B, true, q.N, q.K, q.ldb, 128, 128) || !fs_map(&x, q.A, true, q.M, q.K, q.lda, 128, padded(q.M)))
-        return PAX_ERR_CUDA;
+    FsMaps m;
     FsParams p = {};
     p.M = (int)q.M;
     p.N = (int)q.N;
     p.kbs = (int)((q.K + 127) / 128);
+    p.rows = chunk_rows(q.M);
+    if (!fs_map(&m.w0, q.B, true, q.N, q.K, q.ldb, 128, 128) ||
+        !fs_map(&m.x0, q.A, true, q.M, q.K, q.lda, 128, (uint32_t)p.rows))
+        return PAX_ERR_CUDA;
+    m.w1 = m.w0;
+    m.x1 = m.x0;
     p.C = q.C;
     p.ldc = q.ldc;
     p.sa = q.a_scale, p.sb = q.b_scale, p.bias = q.bias;
     p.c_f16 = q.c_f16;
-    return launch_tokens<FS_I8>(w, w, x, p, stream);
+    return launch_tokens<FS_I8>(m, p, stream);
 }
 
 int read_clear_device_error_ff_skinny() {

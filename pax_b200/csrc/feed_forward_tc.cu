@@ -69,23 +69,25 @@ pax_status_t launch_back_w(const FfMaps& maps, FfParams& p, cudaStream_t stream)
     if (p.x_rem > 0 && p.nw > 0) p.w_extra = (p.kbs + p.kbs_w / 2) / p.kbs_w;
     return ff_launch<FF_BACK, 0, OutT, W>(maps, p, units, stream);
 }
+// The time of both gradients in one launch with tiles of width w.  The weight
+// gradients fill up what dX's tiles leave uneven; a launch ends no earlier
+// than its longest tile.
+double back_time(const FfParams& p, int w, int units) {
+    const double x = p.nx ? tile_cost(w, p.kbs) : 0, y = p.nw ? tile_cost(w, p.kbs_w) : 0;
+    const long long nx = p.nx ? (long long)p.tiles_m * up(p.D, 256 * w) : 0;
+    const long long nw = p.nw ? 2LL * p.wt_m * up(p.F, 256 * w) : 0;
+    double t = p.nx && p.nw ? (nx * x + nw * y) / units + 0.5 * y : rounds(nx, units) * x + rounds(nw, units) * y;
+    if (t < x) t = x;
+    if (t < y) t = y;
+    return t + (w == 1 ? kLastEpilogue : 0);
+}
+
 template <typename OutT>
 pax_status_t launch_back(const FfMaps& maps, FfParams& p, cudaStream_t stream) {
     const int units = ff_units<FF_BACK, 0, OutT, 1>(current_device());
     if (units <= 0) return PAX_ERR_CUDA;
-    // The weight gradients fill up what dX's tiles leave uneven; a launch
-    // ends no earlier than its longest tile.
-    double t[3];
-    for (int w = 1; w <= 2; ++w) {
-        const double x = p.nx ? tile_cost(w, p.kbs) : 0, y = p.nw ? tile_cost(w, p.kbs_w) : 0;
-        const long long nx = p.nx ? (long long)p.tiles_m * up(p.D, 256 * w) : 0;
-        const long long nw = p.nw ? 2LL * p.wt_m * up(p.F, 256 * w) : 0;
-        double even = p.nw ? (nx * x + nw * y) / units + 0.5 * y : rounds(nx, units) * x;
-        if (even < x) even = x;
-        if (even < y) even = y;
-        t[w] = even + (w == 1 ? kLastEpilogue : 0);
-    }
-    return t[2] < t[1] ? launch_back_w<OutT, 2>(maps, p, stream) : launch_back_w<OutT, 1>(maps, p, stream);
+    return back_time(p, 2, units) < back_time(p, 1, units) ? launch_back_w<OutT, 2>(maps, p, stream)
+                                                           : launch_back_w<OutT, 1>(maps, p, stream);
 }
 
 template <typename OutT>
@@ -139,6 +141,30 @@ bool glu_back_tc_ok(const GluGradProblem& q) {
            tiles_ok(up(q.M, 256), up(q.D, 256)) && tiles_ok(up(q.D, 256), 2LL * up(q.F, 256));
 }
 
+static void back_params(const GluGradProblem& q, FfParams& p) {
+    p.M = (int)q.M;
+    p.D = (int)q.D;
+    p.F = (int)q.F;
+    p.N = p.D;
+    p.tiles_m = up(q.M, 256);
+    p.half_kbs = up(q.F, 64);
+    p.kbs = 2 * p.half_kbs;
+    p.group_m = kGroupM;
+    p.wt_m = up(q.D, 256);
+    p.kbs_w = up(q.M, 64);
+    p.nx = q.dX != nullptr;  // counted once the tile width is chosen
+    p.nw = q.dWg != nullptr;
+    p.accumulate = q.accumulate;
+}
+
+double glu_back_tc_time(const GluGradProblem& q) {
+    FfParams p = {};
+    back_params(q, p);
+    const int units = device_sm_count(current_device()) / 2;
+    const double a = back_time(p, 1, units), b = back_time(p, 2, units);
+    return a < b ? a : b;
+}
+
 pax_status_t glu_back_tc(const GluGradProblem& q, cudaStream_t stream) {
     FfMaps maps;
     FfParams p = {};
@@ -159,19 +185,7 @@ pax_status_t glu_back_tc(const GluGradProblem& q, cudaStream_t stream) {
              ff_map(&m[MB_DWG], q.dWg, wt, we, q.D, q.F, q.lddwg, 128 / we, 32) &&
              ff_map(&m[MB_DWU], q.dWu, wt, we, q.D, q.F, q.lddwu, 128 / we, 32);
     if (!ok) return PAX_ERR_CUDA;
-    p.M = (int)q.M;
-    p.D = (int)q.D;
-    p.F = (int)q.F;
-    p.N = p.D;
-    p.tiles_m = up(q.M, 256);
-    p.half_kbs = up(q.F, 64);
-    p.kbs = 2 * p.half_kbs;
-    p.group_m = kGroupM;
-    p.wt_m = up(q.D, 256);
-    p.kbs_w = up(q.M, 64);
-    p.nx = q.dX != nullptr;  // counted once the tile width is chosen
-    p.nw = q.dWg != nullptr;
-    p.accumulate = q.accumulate;
+    back_params(q, p);
     return q.dw_f16 ? launch_back<__half>(maps, p, stream) : launch_back<float>(maps, p, stream);
 }
 

@@ -99,11 +99,13 @@ class _Call:
             if stream != torch.cuda.current_stream(device):
                 self.other = stream
 
-    def empty(self, shape, dtype, scratch=False) -> torch.Tensor:
+    def empty(self, like: torch.Tensor, shape, dtype=None, scratch=False) -> torch.Tensor:
+        if dtype is None:
+            dtype = like.dtype
         if self.other is None:
-            return torch.empty(shape, dtype=dtype, device=self.device)
+            return like.new_empty(shape, dtype=dtype)
         with torch.cuda.stream(self.other):
-            t = torch.empty(shape, dtype=dtype, device=self.device)
+            t = like.new_empty(shape, dtype=dtype)
         if not scratch:
             t.record_stream(torch.cuda.current_stream(self.device))
         return t
@@ -146,9 +148,9 @@ def glu(X: torch.Tensor, Wg: torch.Tensor, Wu: torch.Tensor, *, activation="silu
     if G is not None:
         ldg, ldu = _matrix(G, "G", M, F, _F16, dev), _matrix(U, "U", M, F, _F16, dev)
     call = _Call(dev, stream)
-    H = out if out is not None else call.empty((M, F), torch.float16)
+    H = out if out is not None else call.empty(X, (M, F))
     if save and G is None:
-        G, U = call.empty((M, F), torch.float16), call.empty((M, F), torch.float16)
+        G, U = call.empty(X, (M, F)), call.empty(X, (M, F))
     g, u = (0, 0) if G is None else (G.data_ptr(), U.data_ptr())
     d = _lib.GluDesc(X.data_ptr(), Wg.data_ptr(), Wu.data_ptr(), H.data_ptr(), g, u, M, D, F, ldx, ldwg, ldwu, ldh, ldg,
                      ldu, act)
@@ -188,20 +190,28 @@ def glu_backward(dH: torch.Tensor, X: torch.Tensor, Wg: torch.Tensor, Wu: torch.
         raise ValueError("accumulate needs given float32 dWg and dWu")
     ins = ((dH, "dH", M, F), (X, "X", M, D), (Wg, "Wg", D, F), (Wu, "Wu", D, F), (G, "G", M, F), (U, "U", M, F))
     lds = [_matrix(t, name, r, c, _F16, dev) for t, name, r, c in ins]
-    for t, name, r, c, dt in ((dG, "dG", M, F, _F16), (dU, "dU", M, F, _F16), (dX, "dX", M, D, _F16),
-                              (dWg, "dWg", D, F, (dW_dtype,)), (dWu, "dWu", D, F, (dW_dtype,))):
-        lds.append(c if t is None else _matrix(t, name, r, c, dt, dev))
+    lds += (F if dG is None else _matrix(dG, "dG", M, F, _F16, dev), F if dU is None else _matrix(dU, "dU", M, F, _F16, dev),
+            D if dX is None else _matrix(dX, "dX", M, D, _F16, dev))
+    if dWg is None:
+        lds += (F, F)
+    else:
+        lds += (_matrix(dWg, "dWg", D, F, (dW_dtype,), dev), _matrix(dWu, "dWu", D, F, (dW_dtype,), dev))
     call = _Call(dev, stream)
     if need_dX and dX is None:
-        dX = call.empty((M, D), torch.float16)
+        dX = call.empty(X, (M, D))
     if need_dW and dWg is None:
-        dWg, dWu = call.empty((D, F), dW_dtype), call.empty((D, F), dW_dtype)
-    if dG is None:
-        dG = call.empty((M, F), torch.float16, scratch=True)
-    if dU is None:
-        dU = call.empty((M, F), torch.float16, scratch=True)
-    d = _lib.GluGradDesc(*(0 if t is None else t.data_ptr() for t in (dH, X, Wg, Wu, G, U, dG, dU, dX, dWg, dWu)), M, D, F,
-                         *lds, _DT[dW_dtype], accumulate, act)
+        dWg, dWu = call.empty(Wg, (D, F), dW_dtype), call.empty(Wg, (D, F), dW_dtype)
+    if dG is None and dU is None:
+        scratch = call.empty(X, (2, M, F), scratch=True)  # freed on the call's stream, after the call
+        dg = scratch.data_ptr()
+        du = dg + 2 * M * F
+    else:
+        dG = dG if dG is not None else call.empty(X, (M, F), scratch=True)
+        dU = dU if dU is not None else call.empty(X, (M, F), scratch=True)
+        dg, du = dG.data_ptr(), dU.data_ptr()
+    d = _lib.GluGradDesc(dH.data_ptr(), X.data_ptr(), Wg.data_ptr(), Wu.data_ptr(), G.data_ptr(), U.data_ptr(), dg, du,
+                         *(0 if t is None else t.data_ptr() for t in (dX, dWg, dWu)), M, D, F, *lds, _DT[dW_dtype],
+                         accumulate, act)
     call.run("pax_glu_backward_ex", ctypes.byref(d))
     return dX, dWg, dWu
 
@@ -221,8 +231,8 @@ def quantize_rows(X: torch.Tensor, *, out: torch.Tensor | None = None, scale: to
     if scale is not None:
         _vector(scale, "scale", M, torch.float32, dev)
     call = _Call(dev, stream)
-    Q = out if out is not None else call.empty((M, K), torch.int8)
-    s = scale if scale is not None else call.empty((M,), torch.float32)
+    Q = out if out is not None else call.empty(X, (M, K), torch.int8)
+    s = scale if scale is not None else call.empty(X, (M,), torch.float32)
     call.run("pax_quantize_rows", X.data_ptr(), ldx, Q.data_ptr(), ldq, s.data_ptr(), M, K)
     return Q, s
 
@@ -252,7 +262,7 @@ def gemm_i8(A: torch.Tensor, B: torch.Tensor, a_scale: torch.Tensor, b_scale: to
     elif out_dtype not in _DT:
         raise TypeError("out_dtype must be float32 or float16")
     call = _Call(dev, stream)
-    C = out if out is not None else call.empty((M, N), out_dtype)
+    C = out if out is not None else call.empty(A, (M, N), out_dtype)
     d = _lib.GemmI8Desc(A.data_ptr(), B.data_ptr(), C.data_ptr(), a_scale.data_ptr(), b_scale.data_ptr(),
                         0 if bias is None else bias.data_ptr(), M, N, K, lda, ldb, ldc, _DT[out_dtype])
     call.run("pax_gemm_i8_ex", ctypes.byref(d))
