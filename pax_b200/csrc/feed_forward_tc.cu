@@ -171,20 +171,23 @@ pax_status_t glu_back_tc(const GluGradProblem& q, cudaStream_t stream) {
     CUtensorMap* m = maps.m;
     const CUtensorMapDataType wt = q.dw_f16 ? kF16 : kF32;
     const int we = q.dw_f16 ? 2 : 4;
-    bool ok = ff_map(&m[MB_DGK], q.dG, kF16, 2, q.M, q.F, q.lddg, 64, 128) &&
-              ff_map(&m[MB_DUK], q.dU, kF16, 2, q.M, q.F, q.lddu, 64, 128) &&
-              ff_map(&m[MB_DGN], q.dG, kF16, 2, q.M, q.F, q.lddg, 64, 64) &&
-              ff_map(&m[MB_DUN], q.dU, kF16, 2, q.M, q.F, q.lddu, 64, 64);
-    m[MB_WGK] = m[MB_WUK] = m[MB_DX] = m[MB_XN] = m[MB_DWG] = m[MB_DWU] = m[MB_DGK];
-    if (ok && q.dX)
-        ok = ff_map(&m[MB_WGK], q.Wg, kF16, 2, q.D, q.F, q.ldwg, 64, 128) &&
+    bool ok = true;
+    if (q.dX)
+        ok = ff_map(&m[MB_DGK], q.dG, kF16, 2, q.M, q.F, q.lddg, 64, 128) &&
+             ff_map(&m[MB_DUK], q.dU, kF16, 2, q.M, q.F, q.lddu, 64, 128) &&
+             ff_map(&m[MB_WGK], q.Wg, kF16, 2, q.D, q.F, q.ldwg, 64, 128) &&
              ff_map(&m[MB_WUK], q.Wu, kF16, 2, q.D, q.F, q.ldwu, 64, 128) &&
              ff_map(&m[MB_DX], q.dX, kF16, 2, q.M, q.D, q.lddx, 64, 32);
     if (ok && q.dWg)
-        ok = ff_map(&m[MB_XN], q.X, kF16, 2, q.M, q.D, q.ldx, 64, 64) &&
+        ok = ff_map(&m[MB_DGN], q.dG, kF16, 2, q.M, q.F, q.lddg, 64, 64) &&
+             ff_map(&m[MB_DUN], q.dU, kF16, 2, q.M, q.F, q.lddu, 64, 64) &&
+             ff_map(&m[MB_XN], q.X, kF16, 2, q.M, q.D, q.ldx, 64, 64) &&
              ff_map(&m[MB_DWG], q.dWg, wt, we, q.D, q.F, q.lddwg, 128 / we, 32) &&
              ff_map(&m[MB_DWU], q.dWu, wt, we, q.D, q.F, q.lddwu, 128 / we, 32);
     if (!ok) return PAX_ERR_CUDA;
+    // Maps of what is not computed are never used.
+    if (!q.dX) m[MB_DGK] = m[MB_DUK] = m[MB_WGK] = m[MB_WUK] = m[MB_DX] = m[MB_XN];
+    if (!q.dWg) m[MB_DGN] = m[MB_DUN] = m[MB_XN] = m[MB_DWG] = m[MB_DWU] = m[MB_DX];
     back_params(q, p);
     return q.dw_f16 ? launch_back<__half>(maps, p, stream) : launch_back<float>(maps, p, stream);
 }

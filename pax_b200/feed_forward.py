@@ -188,8 +188,8 @@ def glu_backward(dH: torch.Tensor, X: torch.Tensor, Wg: torch.Tensor, Wu: torch.
         raise TypeError("weight gradients must be float32 or float16")
     if accumulate and (dWg is None or dW_dtype != torch.float32):
         raise ValueError("accumulate needs given float32 dWg and dWu")
-    ins = ((dH, "dH", M, F), (X, "X", M, D), (Wg, "Wg", D, F), (Wu, "Wu", D, F), (G, "G", M, F), (U, "U", M, F))
-    lds = [_matrix(t, name, r, c, _F16, dev) for t, name, r, c in ins]
+    lds = [_matrix(dH, "dH", M, F, _F16, dev), _matrix(X, "X", M, D, _F16, dev), _matrix(Wg, "Wg", D, F, _F16, dev),
+           _matrix(Wu, "Wu", D, F, _F16, dev), _matrix(G, "G", M, F, _F16, dev), _matrix(U, "U", M, F, _F16, dev)]
     lds += (F if dG is None else _matrix(dG, "dG", M, F, _F16, dev), F if dU is None else _matrix(dU, "dU", M, F, _F16, dev),
             D if dX is None else _matrix(dX, "dX", M, D, _F16, dev))
     if dWg is None:
@@ -197,10 +197,14 @@ def glu_backward(dH: torch.Tensor, X: torch.Tensor, Wg: torch.Tensor, Wu: torch.
     else:
         lds += (_matrix(dWg, "dWg", D, F, (dW_dtype,), dev), _matrix(dWu, "dWu", D, F, (dW_dtype,), dev))
     call = _Call(dev, stream)
+    plain = call.other is None  # a contiguous input of the same kind is the quickest model of an output
     if need_dX and dX is None:
-        dX = call.empty(X, (M, D))
+        dX = torch.empty_like(X) if plain and lds[1] == D else call.empty(X, (M, D))
     if need_dW and dWg is None:
-        dWg, dWu = call.empty(Wg, (D, F), dW_dtype), call.empty(Wg, (D, F), dW_dtype)
+        if plain and lds[2] == F and dW_dtype is torch.float16:
+            dWg, dWu = torch.empty_like(Wg), torch.empty_like(Wg)
+        else:
+            dWg, dWu = call.empty(Wg, (D, F), dW_dtype), call.empty(Wg, (D, F), dW_dtype)
     if dG is None and dU is None:
         scratch = call.empty(X, (2, M, F), scratch=True)  # freed on the call's stream, after the call
         dg = scratch.data_ptr()
