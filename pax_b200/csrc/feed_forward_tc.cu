@@ -37,21 +37,50 @@ double tile_cost(int w, int kbs) { return w == 2 ? kbs * kWideBlock + kWideEpilo
 
 int rounds(long long tiles, int units) { return (int)((tiles + units - 1) / units); }
 
-template <int ACT, int W>
-pax_status_t launch_glu_w(const FfMaps& maps, FfParams& p, cudaStream_t stream) {
-    const int most = ff_units<FF_GLU, ACT, __half, W>(current_device());
-    if (most <= 0) return PAX_ERR_CUDA;
-    p.tiles_n = up(p.N, 128 * W);
-    const long long tiles = (long long)p.tiles_m * p.tiles_n;
-    return ff_launch<FF_GLU, ACT, __half, W>(maps, p, (int)(tiles < most ? tiles : most), stream);
+// What a piece of a narrow tile costs: half and quarter widths stage and
+// multiply less per k-block, but A in full, and have a shorter epilogue.
+double piece_cost(int pieces, int kbs) {
+    return pieces == 4 ? 0.6 * kbs + 3.0 : pieces == 2 ? 0.75 * kbs + 5.0 : kbs + kLastEpilogue;
 }
+
+// Whole rounds of narrow tiles, and the rest in the number of column pieces
+// that ends soonest; returns the time.  1235x4099x2064 has 85 tiles on 74
+// pairs: 11 left over.
+double plan_pieces(FfParams& p, int tiles, int units, int most) {
+    const int rest = tiles % units;
+    p.full = tiles - rest;
+    p.pieces = 1;
+    const double whole = (double)(p.full / units) * p.kbs;
+    double best = rest == 0 ? kLastEpilogue : piece_cost(1, p.kbs);
+    for (int n = 2; n <= most && rest > 0; n *= 2) {
+        const double t = rounds((long long)rest * n, units) * piece_cost(n, p.kbs);
+        if (t < best) {
+            best = t;
+            p.pieces = n;
+        }
+    }
+    return whole + best;
+}
+
+int ff_grid(const FfParams& p, int tiles, int units) {
+    const int items = p.full + (tiles - p.full) * p.pieces;
+    return items < units ? items : units;
+}
+
 template <int ACT>
 pax_status_t launch_glu(const FfMaps& maps, FfParams& p, cudaStream_t stream) {
     const int units = ff_units<FF_GLU, ACT, __half, 1>(current_device());
-    if (units <= 0) return PAX_ERR_CUDA;
-    const double t1 = rounds((long long)p.tiles_m * up(p.N, 128), units) * tile_cost(1, p.kbs) + kLastEpilogue;
-    const double t2 = rounds((long long)p.tiles_m * up(p.N, 256), units) * tile_cost(2, p.kbs);
-    return t2 < t1 ? launch_glu_w<ACT, 2>(maps, p, stream) : launch_glu_w<ACT, 1>(maps, p, stream);
+    const int units2 = ff_units<FF_GLU, ACT, __half, 2>(current_device());
+    if (units <= 0 || units2 <= 0) return PAX_ERR_CUDA;
+    p.tiles_n = up(p.N, 128);
+    const int tiles = p.tiles_m * p.tiles_n, tiles2 = p.tiles_m * up(p.N, 256);
+    if (rounds(tiles2, units2) * tile_cost(2, p.kbs) < plan_pieces(p, tiles, units, 2)) {
+        p.tiles_n = up(p.N, 256);
+        p.full = tiles2;
+        p.pieces = 1;
+        return ff_launch<FF_GLU, ACT, __half, 2>(maps, p, tiles2 < units2 ? tiles2 : units2, stream);
+    }
+    return ff_launch<FF_GLU, ACT, __half, 1>(maps, p, ff_grid(p, tiles, units), stream);
 }
 
 template <typename OutT, int W>
@@ -92,11 +121,12 @@ pax_status_t launch_back(const FfMaps& maps, FfParams& p, cudaStream_t stream) {
 
 template <typename OutT>
 pax_status_t launch_i8(const FfMaps& maps, FfParams& p, cudaStream_t stream) {
-    const int most = ff_units<FF_I8, 0, OutT, 1>(current_device());
-    if (most <= 0) return PAX_ERR_CUDA;
+    const int units = ff_units<FF_I8, 0, OutT, 1>(current_device());
+    if (units <= 0) return PAX_ERR_CUDA;
     p.tiles_n = up(p.N, 256);
-    const long long tiles = (long long)p.tiles_m * p.tiles_n;
-    return ff_launch<FF_I8, 0, OutT, 1>(maps, p, (int)(tiles < most ? tiles : most), stream);
+    const int tiles = p.tiles_m * p.tiles_n;
+    plan_pieces(p, tiles, units, 4);
+    return ff_launch<FF_I8, 0, OutT, 1>(maps, p, ff_grid(p, tiles, units), stream);
 }
 
 bool tiles_ok(long long a, long long b) { return a * b <= 0x3fffffffLL; }
@@ -202,7 +232,9 @@ pax_status_t gemm_i8_tc(const I8Problem& q, cudaStream_t stream) {
     CUtensorMap* m = maps.m;
     const int ce = q.c_f16 ? 2 : 4;
     bool ok = ff_map(&m[MI_A], q.A, kU8, 1, q.M, q.K, q.lda, 128, 128) &&
-              ff_map(&m[MI_B], q.B, kU8, 1, q.N, q.K, q.ldb, 128, 128);
+              ff_map(&m[MI_B], q.B, kU8, 1, q.N, q.K, q.ldb, 128, 128) &&
+              ff_map(&m[MI_B2], q.B, kU8, 1, q.N, q.K, q.ldb, 128, 64) &&
+              ff_map(&m[MI_B4], q.B, kU8, 1, q.N, q.K, q.ldb, 128, 32);
     p.c_tma = out16(q.C, q.N, q.ldc, ce);
     m[MI_C] = m[MI_A];
     if (ok && p.c_tma) ok = ff_map(&m[MI_C], q.C, q.c_f16 ? kF16 : kF32, ce, q.M, q.N, q.ldc, 128 / ce, 32);

@@ -41,10 +41,10 @@ enum : int { FF_GLU = 0, FF_BACK = 1, FF_I8 = 2 };
 
 // Tensor maps by role.  FF_GLU: X, Wg, Wu, H, G, U.  FF_BACK: dG, dU, Wg, Wu
 // as rows of a product (K-major), X, dG, dU by columns (MN-major), dX, dWg,
-// dWu.  FF_I8: A, B, C.
+// dWu.  FF_I8: A, B in boxes of 128, 64 and 32 rows, C.
 enum : int { MG_X = 0, MG_WG, MG_WU, MG_H, MG_G, MG_U };
 enum : int { MB_DGK = 0, MB_DUK, MB_WGK, MB_WUK, MB_XN, MB_DGN, MB_DUN, MB_DX, MB_DWG, MB_DWU };
-enum : int { MI_A = 0, MI_B, MI_C };
+enum : int { MI_A = 0, MI_B, MI_B2, MI_B4, MI_C };
 struct FfMaps {
     CUtensorMap m[10];
 };
@@ -54,6 +54,7 @@ struct FfParams {
     int tiles_m, tiles_n;  // output tiles (FF_BACK: of dX)
     int kbs;               // k-blocks of a tile (FF_BACK: of dX, both terms)
     int group_m;           // tiles run in column-major groups of group_m tile rows
+    int full, pieces;      // FF_GLU, FF_I8: tiles [0, full) whole, the others in `pieces` column pieces
     int save;              // FF_GLU: store G and U
     // FF_BACK.  dX is M x D; the weight gradients D x F each, tiles wt_n wide
     // per matrix, both matrices side by side; kbs_w k-blocks of tokens.
@@ -70,6 +71,8 @@ struct FfParams {
 struct FfItem {
     int kind;  // 0 the product (FF_BACK: dX), 1 a weight gradient
     int mb, nb, kbs;
+    int w;     // accumulator columns of one MMA
+    int col;   // FF_GLU, FF_I8: first output column
 };
 
 __host__ __device__ __forceinline__ void ff_tile(int t, int tiles_m, int tiles_n, int group_m, int& mb, int& nb) {
@@ -83,17 +86,28 @@ __host__ __device__ __forceinline__ void ff_tile(int t, int tiles_m, int tiles_n
 
 // The idx-th tile of pair `unit` of `units`; false when there is none.
 // Round-robin, so that the pairs work on neighbouring tiles at a time.
+// FF_GLU and FF_I8: the tiles beyond the last full round can run in column
+// pieces, so that the last round takes less than a whole tile's time.
 // FF_BACK: dX's nx tiles first.  Where they do not divide by the pairs,
 // x_rem pairs have one more, which is worth w_extra weight-gradient tiles;
 // the other pairs start with that many rounds of those.
-template <int MODE>
+template <int MODE, int W>
 __host__ __device__ __forceinline__ bool ff_item(const FfParams& p, int unit, int units, int idx, FfItem& it) {
+    it.w = 256;
     if constexpr (MODE != FF_BACK) {
-        const int t = unit + idx * units;
+        int t = unit + idx * units, piece = 0;
+        if (t >= p.full) {
+            const int j = t - p.full;
+            t = p.full + j / p.pieces;
+            piece = j % p.pieces;
+            it.w = 256 / p.pieces;
+        }
         if (t >= p.tiles_m * p.tiles_n) return false;
         it.kind = 0;
-        it.kbs = p.kbs;
         ff_tile(t, p.tiles_m, p.tiles_n, p.group_m, it.mb, it.nb);
+        const int cols = MODE == FF_GLU ? it.w / 2 : it.w;  // of a piece; the wide tile has no pieces
+        it.col = it.nb * (MODE == FF_GLU ? 128 : 256) * W + piece * cols;
+        it.kbs = it.col < p.N ? p.kbs : 0;  // nothing of a piece beyond the last column
         return true;
     } else {
         const int q = p.nx / units, mine = q + (unit < p.x_rem ? 1 : 0);
@@ -147,6 +161,21 @@ struct FfCfg {
     static_assert(SMEM_BYTES <= 232448, "shared memory budget");
 };
 
+// Columns of a w-wide 8-bit item that each of the two warps of a lane quarter
+// takes: half of them, or all with the first warp where half is less than a
+// 128-byte row of the output.
+template <typename OutT>
+__device__ __forceinline__ int ff_i8_span(int w) {
+    constexpr int row = 128 / (int)sizeof(OutT);
+    return w / 2 >= row ? w / 2 : row;
+}
+
+// Bytes that one CTA stages per k-block of an item.
+template <int W>
+__device__ __forceinline__ uint32_t ff_stage_bytes(const FfItem& it) {
+    return 16384u + (uint32_t)(W * (it.w / 2) * 128);
+}
+
 template <int MODE, int ACT, typename OutT, int W>
 __global__ void __launch_bounds__(FfCfg<MODE, W>::THREADS, 1)
     ff_tc_kernel(const __grid_constant__ FfMaps maps, const __grid_constant__ FfParams p) {
@@ -191,6 +220,7 @@ __global__ void __launch_bounds__(FfCfg<MODE, W>::THREADS, 1)
         *abort_flag = 0;
         fence_mbar_init();
     }
+    if (warp == 2 && lane < (MODE == FF_BACK ? 10 : MODE == FF_I8 ? 5 : 6)) tma_prefetch_desc(&maps.m[lane]);
     if (warp == 1) {
         tmem_alloc<2>(smem_u32(tmem_slot), 512);
         tmem_relinquish<2>();
@@ -209,12 +239,19 @@ __global__ void __launch_bounds__(FfCfg<MODE, W>::THREADS, 1)
             uint32_t phase = 0;
             bool ok = true;
             FfItem it;
-            for (int idx = 0; ok && ff_item<MODE>(p, unit, units, idx, it); ++idx) {
+            for (int idx = 0; ok && ff_item<MODE, W>(p, unit, units, idx, it); ++idx) {
                 const int row = it.mb * 256 + (int)rank * 128;
                 // First column of this CTA's share of B, and from one MMA's
                 // columns to the next one's.
-                const int col = MODE == FF_GLU ? it.nb * 128 * W : it.nb * 256 * W + (int)rank * 128;
-                constexpr int next = MODE == FF_GLU ? 128 : 256;
+                const int col = MODE == FF_GLU ? it.col
+                                : MODE == FF_I8 ? it.col + (int)rank * (it.w / 2)
+                                                : it.nb * 256 * W + (int)rank * 128;
+                const uint32_t bytes = ff_stage_bytes<W>(it);
+                const CUtensorMap* m_b = MODE == FF_GLU   ? &maps.m[leader ? MG_WG : MG_WU]
+                                         : MODE == FF_I8 ? &maps.m[it.w == 256 ? MI_B : it.w == 128 ? MI_B2 : MI_B4]
+                                                         : nullptr;
+                const int boxes = it.w / 128 * W;  // FF_GLU: 64-column boxes
+                constexpr int next = 256;
                 for (int kb = 0; kb < it.kbs; ++kb) {
                     if (!mbar_wait(empty0 + 8u * stage, phase ^ 1u, abort_flag)) {
                         ok = false;
@@ -223,18 +260,16 @@ __global__ void __launch_bounds__(FfCfg<MODE, W>::THREADS, 1)
                     const uint32_t fb = mapa_shared(full0 + 8u * stage, 0);
                     const uint32_t a = smem_u32(sA + stage * Cfg::A_BYTES), b = smem_u32(sB + stage * Cfg::B_BYTES);
                     // Both CTAs' loads complete on the even CTA's barrier.
-                    if (leader) mbar_arrive_expect_tx(full0 + 8u * stage, 2 * Cfg::STAGE_BYTES);
+                    if (leader) mbar_arrive_expect_tx(full0 + 8u * stage, 2 * bytes);
                     const int k = kb * KB;
                     if constexpr (MODE == FF_GLU) {
-                        const CUtensorMap* w = &maps.m[leader ? MG_WG : MG_WU];
                         tma_load_3d_pair(a, &maps.m[MG_X], fb, k, row, 0);
 #pragma unroll
-                        for (int h = 0; h < 2 * W; ++h) tma_load_3d_pair(b + h * 8192, w, fb, col + 64 * h, k, 0);
+                        for (int h = 0; h < 2 * W; ++h)
+                            if (h < boxes) tma_load_3d_pair(b + h * 8192, m_b, fb, col + 64 * h, k, 0);
                     } else if constexpr (MODE == FF_I8) {
                         tma_load_3d_pair(a, &maps.m[MI_A], fb, k, row, 0);
-#pragma unroll
-                        for (int h = 0; h < W; ++h)
-                            tma_load_3d_pair(b + h * Cfg::OP_BYTES, &maps.m[MI_B], fb, k, col + next * h, 0);
+                        tma_load_3d_pair(b, m_b, fb, k, col, 0);
                     } else if (it.kind == 0) {
                         const bool up = kb >= p.half_kbs;
                         const int kk = up ? k - p.half_kbs * KB : k;
@@ -281,8 +316,15 @@ __global__ void __launch_bounds__(FfCfg<MODE, W>::THREADS, 1)
                 const int most = total > theirs ? total : theirs;
                 for (int s = 0; s < STAGES && s < most; ++s) {
                     const int i = s + ((most - 1 - s) / STAGES) * STAGES;  // last k-block on slot s
-                    if (i < total && i >= theirs) mbar_complete_tx(full0 + 8u * s, Cfg::STAGE_BYTES);
-                    if (i >= total && i < theirs) mbar_arrive_expect_tx(full0 + 8u * s, Cfg::STAGE_BYTES);
+                    if ((i < total) != (i < theirs)) {
+                        int left = i;  // the item that k-block i belongs to
+                        for (int idx = 0; ff_item<MODE, W>(p, unit, units, idx, it) && left >= it.kbs; ++idx)
+                            left -= it.kbs;
+                        if (i < total)
+                            mbar_complete_tx(full0 + 8u * s, ff_stage_bytes<W>(it));
+                        else
+                            mbar_arrive_expect_tx(full0 + 8u * s, ff_stage_bytes<W>(it));
+                    }
                     mbar_wait(full0 + 8u * s, (uint32_t)(i / STAGES) & 1u, nullptr);
                 }
             }
@@ -299,12 +341,13 @@ __global__ void __launch_bounds__(FfCfg<MODE, W>::THREADS, 1)
             const uint64_t aK = umma_desc_sw128(smem_u32(sA), 16, 1024), aN = umma_desc_sw128(smem_u32(sA), 8192, 1024);
             const uint64_t bK = umma_desc_sw128(smem_u32(sB), 16, 1024), bN = umma_desc_sw128(smem_u32(sB), 8192, 1024);
             FfItem it;
-            for (int idx = 0; ok && ff_item<MODE>(p, unit, units, idx, it); ++idx) {
+            for (int idx = 0; ok && ff_item<MODE, W>(p, unit, units, idx, it); ++idx) {
                 const bool a_n = MODE == FF_BACK && it.kind == 1;
                 const bool b_n = MODE == FF_GLU || a_n;
                 const uint64_t a0 = a_n ? aN : aK, b0 = b_n ? bN : bK;
                 const uint64_t a_step = a_n ? 128 : 2, b_step = b_n ? 128 : 2;
-                const uint32_t id = MODE == FF_I8 ? umma_idesc_i8(256, 256) : umma_idesc_f16(256, 256, a_n, b_n);
+                const uint32_t id = MODE == FF_I8 ? umma_idesc_i8(256, it.w) : umma_idesc_f16(256, it.w, a_n, b_n);
+                if (it.kbs == 0) continue;
                 // Releases come from both CTAs' epilogues.
                 if (!mbar_wait<true>(tempty0 + 8u * acc, acc_phase ^ 1u, abort_flag)) break;
                 tc_fence_after();
@@ -384,18 +427,20 @@ __global__ void __launch_bounds__(FfCfg<MODE, W>::THREADS, 1)
         int acc = 0;
         uint32_t acc_phase = 0;
         FfItem it;
-        for (int idx = 0; ff_item<MODE>(p, unit, units, idx, it); ++idx) {
+        for (int idx = 0; ff_item<MODE, W>(p, unit, units, idx, it); ++idx) {
+            if (it.kbs == 0) continue;
             const int row0 = it.mb * 256 + (int)rank * 128 + q * 32;
             float* tab = sTab + (warp - 2) * 256;  // this warp's 128 scales, then its 128 bias values
             float sa = 0.f;
             if constexpr (MODE == FF_I8) {
                 if (row0 + lane < p.M) sa = __ldg(p.sa + row0 + lane);
-                const int c0 = it.nb * 256 + wh * 128 + lane;
+                const int span = ff_i8_span<OutT>(it.w), c0 = it.col + wh * span + lane;
 #pragma unroll
                 for (int i = 0; i < 128; i += 32) {
                     const int c = c0 + i;
-                    tab[lane + i] = c < p.N ? __ldg(p.sb + c) : 0.f;
-                    tab[128 + lane + i] = p.bias && c < p.N ? __half2float(p.bias[c]) : 0.f;
+                    const bool in = i < span && c < p.N;
+                    tab[lane + i] = in ? __ldg(p.sb + c) : 0.f;
+                    tab[128 + lane + i] = in && p.bias ? __half2float(p.bias[c]) : 0.f;
                 }
                 __syncwarp();
             }
@@ -415,19 +460,21 @@ __global__ void __launch_bounds__(FfCfg<MODE, W>::THREADS, 1)
                 }
             };
             if constexpr (MODE == FF_GLU) {
-                // 64 columns of H per warp and MMA: G beside U.
-                const int chunks = row0 >= p.M ? 0 : min(W, max(0, (p.N - it.nb * 128 * W - wh * 64 + 127) / 128));
+                // 64 columns of H per warp and MMA: G beside U
+                // (half a tile: all of them with the first warp).
+                const int here = p.N - it.col - wh * 64;
+                const int chunks = row0 >= p.M || (it.w < 256 && wh == 1) ? 0 : min(W, max(0, (here + 127) / 128));
                 if (chunks == 0) release();
 #pragma unroll 1
                 for (int n = 0; n < chunks; ++n) {
-                    const int col = it.nb * 128 * W + n * 128 + wh * 64;
+                    const int col = it.col + n * 128 + wh * 64;
                     const uint32_t t_gu = t_row + (uint32_t)(n * 256 + wh * 64);
                     uint32_t wH[32], wG[32], wU[32];
 #pragma unroll
                     for (int h = 0; h < 2; ++h) {
                         float g[32], u[32];
                         tmem_ld_32x32b_x32(t_gu + (uint32_t)(32 * h), g);
-                        tmem_ld_32x32b_x32(t_gu + (uint32_t)(128 + 32 * h), u);
+                        tmem_ld_32x32b_x32(t_gu + (uint32_t)(it.w / 2 + 32 * h), u);
                         tmem_wait_ld();
                         if (h == 1 && n == chunks - 1) release();
 #pragma unroll
@@ -445,13 +492,16 @@ __global__ void __launch_bounds__(FfCfg<MODE, W>::THREADS, 1)
                     }
                 }
             } else {
-                // 128 W columns per warp, in chunks of one 128-byte row a lane.
+                // Half of the columns per warp (128 W of whole tiles), in chunks
+                // of one 128-byte row a lane.
                 const bool f16 = sizeof(OutT) == 2 || (MODE == FF_BACK && it.kind == 0);
                 const bool up = MODE == FF_BACK && it.kind == 1 && it.nb >= p.wt_n;
                 const int rows = MODE == FF_BACK ? (it.kind == 0 ? p.M : p.D) : p.M;
                 const int cols = MODE == FF_BACK ? (it.kind == 0 ? p.D : p.F) : p.N;
-                const int tcol = (up ? it.nb - p.wt_n : it.nb) * 256 * W + wh * 128 * W;
-                const int valid = row0 < rows ? min(128 * W, cols - tcol) : 0;
+                const int span = MODE == FF_I8 ? ff_i8_span<OutT>(it.w) : 128 * W;
+                const int base = MODE == FF_I8 ? it.col : (up ? it.nb - p.wt_n : it.nb) * 256 * W;
+                const int tcol = base + wh * span;
+                const int valid = row0 < rows && wh * span < it.w * W ? min(span, cols - tcol) : 0;
                 const int nsub = valid > 0 ? (valid + 31) / 32 : 0;  // 32-column parts that hold anything
                 const CUtensorMap* m = MODE == FF_I8 ? &maps.m[MI_C]
                                                      : &maps.m[it.kind == 0 ? MB_DX : up ? MB_DWU : MB_DWG];
@@ -461,7 +511,7 @@ __global__ void __launch_bounds__(FfCfg<MODE, W>::THREADS, 1)
 #pragma unroll 1
                 for (int s = 0; s < nsub; ++s) {
                     float v[32];
-                    tmem_ld_32x32b_x32(t_row + (uint32_t)(wh * 128 * W + 32 * s), v);
+                    tmem_ld_32x32b_x32(t_row + (uint32_t)(wh * span + 32 * s), v);
                     tmem_wait_ld();
                     if (s == nsub - 1) release();
                     const int col = tcol + 32 * s;
@@ -538,7 +588,7 @@ __global__ void __launch_bounds__(FfCfg<MODE, W>::THREADS, 1)
                 acc_phase ^= 1u;
             }
         }
-        if (lane == 0) bulk_wait<0>();
+        if (lane == 0) bulk_wait_read<0>();  // the staging buffer outlives its last store's read
         __syncwarp();
     }
 
