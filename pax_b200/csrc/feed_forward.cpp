@@ -46,6 +46,13 @@ pax_status_t device_ok(const char* who) {
     return PAX_OK;
 }
 
+// Beyond 64 tokens: whether chunks of 64 on the few-token kernel, which
+// splits K, end sooner than tiles of 256 rows.  Both times come in k-blocks of
+// 0.36 us; a chunk's k-block also carries 64 tokens (0.47 us) and the kernel
+// about 5 us besides.  8-bit 128x4096x4096 takes 12.7 us in chunks and 15.3
+// in tiles, 256x1024x4096 10.8 and 14.2, but 128x11264x4096 24.0 and 17.5.
+bool chunks_pay(double chunks, double tiles) { return 1.15 * (0.47 * chunks + 5.0) < 0.36 * tiles + 1.0; }
+
 pax_status_t done(pax_status_t st, const char* who) {
     if (st == PAX_OK) return report_status(PAX_OK, "");
     return refuse(st, "%s: launch failed (%s)", who, pax_status_string(st));
@@ -167,7 +174,10 @@ pax_status_t pax_glu_ex(const pax_glu_desc_t* desc, cudaStream_t stream) {
     if (st != PAX_OK) return st;
     if (p.M == 0 || p.F == 0) return report_status(PAX_OK, "");
     if ((st = device_ok("pax_glu_ex")) != PAX_OK) return st;
-    st = glu_skinny_ok(p) ? glu_skinny(p, stream) : glu_tc_ok(p) ? glu_tc(p, stream) : glu_any(p, stream);
+    const bool few = glu_skinny_ok(p), tc = glu_tc_ok(p);
+    st = few && (p.M <= 64 || !tc || chunks_pay(glu_skinny_time(p), glu_tc_time(p))) ? glu_skinny(p, stream)
+         : tc                                                                         ? glu_tc(p, stream)
+                                                                                      : glu_any(p, stream);
     return done(st, "pax_glu_ex");
 }
 
@@ -229,9 +239,10 @@ pax_status_t pax_gemm_i8_ex(const pax_gemm_i8_desc_t* desc, cudaStream_t stream)
     if (st != PAX_OK) return st;
     if (p.M == 0 || p.N == 0) return report_status(PAX_OK, "");
     if ((st = device_ok("pax_gemm_i8_ex")) != PAX_OK) return st;
-    st = gemm_i8_skinny_ok(p) ? gemm_i8_skinny(p, stream)
-         : gemm_i8_tc_ok(p)   ? gemm_i8_tc(p, stream)
-                              : gemm_i8_any(p, stream);
+    const bool few = gemm_i8_skinny_ok(p), tc = gemm_i8_tc_ok(p);
+    st = few && (p.M <= 64 || !tc || chunks_pay(gemm_i8_skinny_time(p), gemm_i8_tc_time(p))) ? gemm_i8_skinny(p, stream)
+         : tc                                                                               ? gemm_i8_tc(p, stream)
+                                                                                            : gemm_i8_any(p, stream);
     return done(st, "pax_gemm_i8_ex");
 }
 

@@ -43,27 +43,30 @@ pax_status_t glu_dw_any(const GluGradProblem& p, cudaStream_t stream);
 pax_status_t gemm_i8_any(const I8Problem& p, cudaStream_t stream);
 
 // feed_forward_tc.cu: tcgen05 kernels; *_ok says whether the problem's
-// layout lets them.  glu_back_tc takes dG and dU as glu_grad_rows left them.
+// layout lets them, *_time how long they are expected to take, in k-blocks of
+// about 0.36 us.  glu_back_tc takes dG and dU as glu_grad_rows left them.
 bool glu_tc_ok(const GluProblem& p);
+double glu_tc_time(const GluProblem& p);
 pax_status_t glu_tc(const GluProblem& p, cudaStream_t stream);
 bool glu_back_tc_ok(const GluGradProblem& p);
 double glu_back_tc_time(const GluGradProblem& p);
 pax_status_t glu_back_tc(const GluGradProblem& p, cudaStream_t stream);
 bool gemm_i8_tc_ok(const I8Problem& p);
+double gemm_i8_tc_time(const I8Problem& p);
 pax_status_t gemm_i8_tc(const I8Problem& p, cudaStream_t stream);
 int read_clear_device_error_ff_tc();
 bool set_wait_limit_ff_tc(unsigned long long ns);
 
-// feed_forward_skinny.cu: the gated and the 8-bit product of at most 64
-// tokens; the input gradient of any number, with its modelled time in
-// k-blocks (about 0.36 us each), as glu_back_tc_time's for the tiles of
-// glu_back_tc.
+// feed_forward_skinny.cu: few tokens, in chunks of at most 64 (the gated and
+// the 8-bit product up to 512), with the same kind of expectation.
 bool glu_dx_skinny_ok(const GluGradProblem& p);
 double glu_dx_skinny_time(const GluGradProblem& p);
 pax_status_t glu_dx_skinny(const GluGradProblem& p, cudaStream_t stream);
 bool glu_skinny_ok(const GluProblem& p);
+double glu_skinny_time(const GluProblem& p);
 pax_status_t glu_skinny(const GluProblem& p, cudaStream_t stream);
 bool gemm_i8_skinny_ok(const I8Problem& p);
+double gemm_i8_skinny_time(const I8Problem& p);
 pax_status_t gemm_i8_skinny(const I8Problem& p, cudaStream_t stream);
 int read_clear_device_error_ff_skinny();
 bool set_wait_limit_ff_skinny(unsigned long long ns);

@@ -409,6 +409,15 @@ pax_status_t launch_tokens(const FsMaps& m, const FsParams& p, cudaStream_t stre
     return launch_skinny<MODE, 64>(m, p, stream);
 }
 
+template <int MODE>
+double plan_time(const FsParams& p) {
+    const double t = p.rows <= 16   ? fs_plan<MODE, 16>(p).time
+                     : p.rows <= 32 ? fs_plan<MODE, 32>(p).time
+                     : p.rows <= 48 ? fs_plan<MODE, 48>(p).time
+                                    : fs_plan<MODE, 64>(p).time;
+    return t < 0 ? 1e30 : t;
+}
+
 // Equal chunks of at most 64 tokens.
 int chunk_rows(long long M) {
     const long long chunks = (M + 63) / 64;
@@ -421,17 +430,30 @@ bool rows16(const void* p, long long ld, int elem) {
 
 }  // namespace
 
+// More tokens than this never read the weights again for another chunk.
+constexpr long long kMaxChunked = 512;
+
 bool glu_skinny_ok(const GluProblem& q) {
-    return q.M <= 64 && q.D > 0 && rows16(q.X, q.ldx, 2) && rows16(q.Wg, q.ldwg, 2) && rows16(q.Wu, q.ldwu, 2);
+    return q.M <= kMaxChunked && q.D > 0 && rows16(q.X, q.ldx, 2) && rows16(q.Wg, q.ldwg, 2) && rows16(q.Wu, q.ldwu, 2);
+}
+
+static void glu_params(const GluProblem& q, FsParams& p) {
+    p.M = (int)q.M;
+    p.N = (int)q.F;
+    p.kbs = (int)((q.D + 63) / 64);
+    p.rows = chunk_rows(q.M);
+}
+
+double glu_skinny_time(const GluProblem& q) {
+    FsParams p = {};
+    glu_params(q, p);
+    return plan_time<FS_GLU>(p);
 }
 
 pax_status_t glu_skinny(const GluProblem& q, cudaStream_t stream) {
     FsMaps m;
     FsParams p = {};
-    p.M = (int)q.M;
-    p.N = (int)q.F;
-    p.kbs = (int)((q.D + 63) / 64);
-    p.rows = chunk_rows(q.M);
+    glu_params(q, p);
     if (!fs_map(&m.w0, q.Wg, false, q.D, q.F, q.ldwg, 64, 64) || !fs_map(&m.w1, q.Wu, false, q.D, q.F, q.ldwu, 64, 64) ||
         !fs_map(&m.x0, q.X, false, q.M, q.D, q.ldx, 64, (uint32_t)p.rows))
         return PAX_ERR_CUDA;
@@ -460,11 +482,7 @@ static void dx_params(const GluGradProblem& q, FsParams& p) {
 double glu_dx_skinny_time(const GluGradProblem& q) {
     FsParams p = {};
     dx_params(q, p);
-    const double t = p.rows <= 16   ? fs_plan<FS_DX, 16>(p).time
-                     : p.rows <= 32 ? fs_plan<FS_DX, 32>(p).time
-                     : p.rows <= 48 ? fs_plan<FS_DX, 48>(p).time
-                                    : fs_plan<FS_DX, 64>(p).time;
-    return t < 0 ? 1e30 : t;
+    return plan_time<FS_DX>(p);
 }
 
 pax_status_t glu_dx_skinny(const GluGradProblem& q, cudaStream_t stream) {
@@ -479,16 +497,26 @@ pax_status_t glu_dx_skinny(const GluGradProblem& q, cudaStream_t stream) {
 }
 
 bool gemm_i8_skinny_ok(const I8Problem& q) {
-    return q.M <= 64 && q.K > 0 && rows16(q.A, q.lda, 1) && rows16(q.B, q.ldb, 1);
+    return q.M <= kMaxChunked && q.K > 0 && rows16(q.A, q.lda, 1) && rows16(q.B, q.ldb, 1);
+}
+
+static void i8_params(const I8Problem& q, FsParams& p) {
+    p.M = (int)q.M;
+    p.N = (int)q.N;
+    p.kbs = (int)((q.K + 127) / 128);
+    p.rows = chunk_rows(q.M);
+}
+
+double gemm_i8_skinny_time(const I8Problem& q) {
+    FsParams p = {};
+    i8_params(q, p);
+    return plan_time<FS_I8>(p);
 }
 
 pax_status_t gemm_i8_skinny(const I8Problem& q, cudaStream_t stream) {
     FsMaps m;
     FsParams p = {};
-    p.M = (int)q.M;
-    p.N = (int)q.N;
-    p.kbs = (int)((q.K + 127) / 128);
-    p.rows = chunk_rows(q.M);
+    i8_params(q, p);
     if (!fs_map(&m.w0, q.B, true, q.N, q.K, q.ldb, 128, 128) ||
         !fs_map(&m.x0, q.A, true, q.M, q.K, q.lda, 128, (uint32_t)p.rows))
         return PAX_ERR_CUDA;

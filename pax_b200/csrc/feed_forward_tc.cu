@@ -139,6 +139,19 @@ bool glu_tc_ok(const GluProblem& q) {
            tiles_ok(up(q.M, 256), up(q.F, 128));
 }
 
+// Few tiles read their operands from DRAM at the pace of the ring's depth, a
+// k-block in 0.36 us however narrow its piece.
+static double cold_tiles(double time, int kbs) { return time < kbs + kLastEpilogue ? kbs + kLastEpilogue : time; }
+
+double glu_tc_time(const GluProblem& q) {
+    FfParams p = {};
+    p.kbs = up(q.D, 64);
+    const int units = device_sm_count(current_device()) / 2, tm = up(q.M, 256);
+    const double wide = rounds((long long)tm * up(q.F, 256), units) * tile_cost(2, p.kbs);
+    const double narrow = cold_tiles(plan_pieces(p, tm * up(q.F, 128), units, 2), p.kbs);
+    return wide < narrow ? wide : narrow;
+}
+
 pax_status_t glu_tc(const GluProblem& q, cudaStream_t stream) {
     FfMaps maps;
     FfParams p = {};
@@ -224,6 +237,12 @@ pax_status_t glu_back_tc(const GluGradProblem& q, cudaStream_t stream) {
 
 bool gemm_i8_tc_ok(const I8Problem& q) {
     return q.K > 0 && rows16(q.A, q.lda, 1) && rows16(q.B, q.ldb, 1) && tiles_ok(up(q.M, 256), up(q.N, 256));
+}
+
+double gemm_i8_tc_time(const I8Problem& q) {
+    FfParams p = {};
+    p.kbs = up(q.K, 128);
+    return cold_tiles(plan_pieces(p, up(q.M, 256) * up(q.N, 256), device_sm_count(current_device()) / 2, 4), p.kbs);
 }
 
 pax_status_t gemm_i8_tc(const I8Problem& q, cudaStream_t stream) {
