@@ -293,7 +293,7 @@ pax_status_t pax_ipc_close(void* device_ptr);
  * that serves quantised weights.  All calls are asynchronous on `stream`,
  * allocate nothing and keep nothing between calls, so any number of them may
  * run at once and be captured into graphs.  Zero leading dimensions mean
- * contiguous.  Dimensions are below 2^31.  Outputs must not overlap inputs or
+ * contiguous.  Dimensions are below 2^31 - 1024.  Outputs must not overlap inputs or
  * one another, except where a field says so.  Bases and row pitches that are
  * multiples of 16 bytes run on the tcgen05 / TMA kernels; any other layout
  * runs on a slower kernel with the same results.

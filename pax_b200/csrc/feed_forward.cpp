@@ -19,7 +19,8 @@ pax_status_t refuse(pax_status_t s, const char* fmt, ...) {
     return report_status(s, msg);
 }
 
-constexpr long long kMaxDim = 0x7fffffffLL;
+// Room for the kernels' rounded-up tile coordinates in 32 bits.
+constexpr long long kMaxDim = 0x7fffffffLL - 1024;
 
 bool dim_ok(long long v) { return v >= 0 && v <= kMaxDim; }
 
@@ -126,6 +127,17 @@ pax_status_t check_grad(const pax_glu_grad_desc_t* d, GluGradProblem* p) {
         (dw && (!matrix_ok_sized(p->dWg, p->dw_f16 ? 2 : 4, p->D, p->F, &p->lddwg) ||
                 !matrix_ok_sized(p->dWu, p->dw_f16 ? 2 : 4, p->D, p->F, &p->lddwu))))
         return refuse(PAX_ERR_INVALID, "%s: NULL or misaligned operand, or leading dimension smaller than the row length", who);
+    // In place means element by element: one buffer, one pitch.
+    const struct {
+        const __half* base;
+        long long ld;
+    } outs[2] = {{p->dG, p->lddg}, {p->dU, p->lddu}}, ins[3] = {{p->dH, p->lddh}, {p->G, p->ldg}, {p->U, p->ldu}};
+    for (const auto& o : outs)
+        for (const auto& i : ins)
+            if (p->M > 1 && p->F > 0 && o.base == i.base && o.ld != i.ld)
+                return refuse(PAX_ERR_INVALID, "%s: dG or dU in place of an input needs its leading dimension", who);
+    if (p->M > 0 && p->F > 0 && p->dG == p->dU)
+        return refuse(PAX_ERR_INVALID, "%s: dG and dU are one buffer", who);
     return PAX_OK;
 }
 

@@ -278,10 +278,18 @@ bool fs_map(CUtensorMap* m, const void* base, bool i8, long long rows, long long
 constexpr int kMaxSplit = 8;
 
 
+// Allow the kernel its shared memory on the current device: per device and
+// context, and cheap to repeat.
+template <int MODE, int MP, int R>
+bool fs_shared() {
+    return cudaFuncSetAttribute(ff_skinny_kernel<MODE, MP, R>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                (int)FsCfg<MODE, MP, R>::SMEM_BYTES) == cudaSuccess;
+}
+
 // Clusters of S CTAs that device `dev` holds at once: R times what it holds
 // with one CTA per SM, which is what the runtime answers (a cluster's CTAs
-// share a GPC, so this can be below the SMs' room).  Also sets the kernel's
-// shared-memory limit there.  Asked once per device, kernel and S; 0: error.
+// share a GPC, so this can be below the SMs' room).  Asked once per device,
+// kernel and S; 0: error.
 template <int MODE, int MP, int R>
 int fs_clusters(int dev, int S) {
     static int cache[64][kMaxSplit + 1] = {{0}};
@@ -289,9 +297,7 @@ int fs_clusters(int dev, int S) {
     if (v == 0) {
         using Cfg = FsCfg<MODE, MP, R>;
         auto kern = ff_skinny_kernel<MODE, MP, R>;
-        if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)Cfg::SMEM_BYTES) !=
-            cudaSuccess)
-            return 0;
+        if (!fs_shared<MODE, MP, R>()) return 0;
         cudaLaunchConfig_t cfg = {};
         cudaLaunchAttribute attr[1];
         attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -320,6 +326,7 @@ struct FsMaps {
 template <int MODE, int MP, int R>
 pax_status_t launch_split(const FsMaps& m, const FsParams& p, long long tiles, int S, cudaStream_t stream) {
     using Cfg = FsCfg<MODE, MP, R>;
+    if (!fs_shared<MODE, MP, R>()) return PAX_ERR_CUDA;
     cudaLaunchConfig_t cfg = {};
     cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;

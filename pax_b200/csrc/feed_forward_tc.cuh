@@ -588,7 +588,7 @@ __global__ void __launch_bounds__(FfCfg<MODE, W>::THREADS, 1)
                 acc_phase ^= 1u;
             }
         }
-        if (lane == 0) bulk_wait_read<0>();  // the staging buffer outlives its last store's read
+        if (lane == 0) bulk_wait<0>();
         __syncwarp();
     }
 
@@ -620,18 +620,24 @@ inline bool ff_map(CUtensorMap* m, const void* base, CUtensorMapDataType dt, int
                CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
+// Allow the kernel its shared memory on the current device: per device and
+// context, and cheap to repeat.
+template <int MODE, int ACT, typename OutT, int W>
+inline bool ff_shared() {
+    return cudaFuncSetAttribute(ff_tc_kernel<MODE, ACT, OutT, W>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                (int)FfCfg<MODE, W>::SMEM_BYTES) == cudaSuccess;
+}
+
 // CTA pairs of the kernel that device `dev` holds at once (SMs pair up
-// within a GPC, so this can be below SMs / 2).  Also sets the kernel's
-// shared-memory limit there; asked once per device and kernel.
+// within a GPC, so this can be below SMs / 2); asked once per device and
+// kernel.
 template <int MODE, int ACT, typename OutT, int W>
 inline int ff_units(int dev) {
     static int cache[64] = {0};
     int& v = cache[dev & 63];
     if (v == 0) {
         auto kern = ff_tc_kernel<MODE, ACT, OutT, W>;
-        if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)FfCfg<MODE, W>::SMEM_BYTES) !=
-            cudaSuccess)
-            return 0;
+        if (!ff_shared<MODE, ACT, OutT, W>()) return 0;
         const int sms = device_sm_count(dev);
         cudaLaunchConfig_t cfg = {};
         cudaLaunchAttribute attr[1];
@@ -656,6 +662,7 @@ inline int ff_units(int dev) {
 
 template <int MODE, int ACT, typename OutT, int W>
 inline pax_status_t ff_launch(const FfMaps& maps, const FfParams& p, int units, cudaStream_t stream) {
+    if (!ff_shared<MODE, ACT, OutT, W>()) return PAX_ERR_CUDA;
     cudaLaunchConfig_t cfg = {};
     cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;

@@ -123,11 +123,14 @@ def test_pax_glu_ex_refusals(bad):
     assert call("pax_glu_ex", filled(_lib.GluDesc, **{"M": 4, "D": 16, "F": 8, **bad})) == INVALID
 
 
-@pytest.mark.parametrize("bad", [{"M": -1}, {"act": 3}, {"dH": None}, {"X": None}, {"Wg": None}, {"G": None}, {"dG": None}, {"dU": None},
+GRAD_PTRS = {"dU": 128, "dX": 192, "dWg": 256, "dWu": 320}
+
+
+@pytest.mark.parametrize("bad", [{"dG": 128}, {"lddg": 16}, {"dG": 192, "dU": 64, "ldg": 16}, {"M": -1}, {"act": 3}, {"dH": None}, {"X": None}, {"Wg": None}, {"G": None}, {"dG": None}, {"dU": None},
                                  {"dWg": None}, {"dWu": None}, {"dw_dtype": 2}, {"dw_dtype": 1, "accumulate": 1}, {"lddh": 7},
                                  {"lddwg": 7}, {"dWg": 66}])
 def test_pax_glu_backward_ex_refusals(bad):
-    assert call("pax_glu_backward_ex", filled(_lib.GluGradDesc, **{"M": 4, "D": 16, "F": 8, **bad})) == INVALID
+    assert call("pax_glu_backward_ex", filled(_lib.GluGradDesc, **{"M": 4, "D": 16, "F": 8, **GRAD_PTRS, **bad})) == INVALID
 
 
 @pytest.mark.parametrize("bad", [{"M": -1}, {"K": 131072}, {"A": None}, {"B": None}, {"C": None}, {"a_scale": None}, {"b_scale": None},
