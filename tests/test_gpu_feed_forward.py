@@ -455,5 +455,37 @@ def test_other_stream_and_calls_at_once(gen, M):
                 assert torch.equal(a, b)
 
 
+CAPTURE_FIRST = """
+import torch, pax_b200
+g = torch.Generator(device="cuda"); g.manual_seed(3)
+h = lambda *s: (torch.randn(s, generator=g, device="cuda") * 0.1).half()
+for M in (7, 300):
+    X, Wg, Wu, dH = h(M, 264), h(264, 520), h(264, 520), h(M, 520)
+    Wq, sw = torch.randint(-9, 9, (136, 264), device="cuda", dtype=torch.int8), torch.rand(136, device="cuda")
+    def run():
+        H, G, U = pax_b200.glu(X, Wg, Wu, save=True)
+        Q, s = pax_b200.quantize_rows(X)
+        return (H, G, U, *pax_b200.glu_backward(dH, X, Wg, Wu, G, U), Q, s, pax_b200.gemm_i8(Q, Wq, s, sw))
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = run()
+    graph.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(out, run()))
+print("ok")
+"""
+
+
+def test_the_first_call_of_a_process_can_be_captured(cuda):
+    import os
+    import subprocess
+    import sys
+
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    r = subprocess.run([sys.executable, "-c", CAPTURE_FIRST], cwd=root, capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0 and r.stdout.strip().endswith("ok"), r.stderr[-2000:]
+
+
 def test_no_device_error_was_recorded(cuda):
     assert pax_b200.device_error() == pax_b200.Status.OK
