@@ -3,8 +3,10 @@
 Compiles each translation unit under ``pax_b200/csrc`` with nvcc
 (``-gencode arch=compute_100a,code=sm_100a -lineinfo``) into
 ``pax_b200/_build`` and links them into one shared library next to this
-file, so the library travels with the source tree.  Objects are rebuilt when
-any source or header is newer.  Run ``python -m pax_b200.build``.
+file, so the library travels with the source tree.  The feed-forward
+products' binding to torch tensors, ``pax_b200/_feed_forward.so``, is compiled
+with g++ against the installed torch and linked to that library.  Objects are
+rebuilt when any source or header is newer.  Run ``python -m pax_b200.build``.
 """
 from __future__ import annotations
 
@@ -13,11 +15,13 @@ import glob
 import os
 import subprocess
 import sys
+import sysconfig
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 BUILD_DIR = os.path.join(HERE, "_build")
 LIB = os.path.join(HERE, "libpax_b200.so")
+TORCH_LIB = os.path.join(HERE, "_feed_forward.so")
 INCLUDE = os.path.join(os.path.dirname(HERE), "include")
 NVCC = os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc")
 
@@ -75,7 +79,31 @@ def build(force: bool = False, verbose: bool = False) -> str:
         if r.returncode != 0:
             raise RuntimeError(f"link failed:\n{r.stdout}\n{r.stderr}")
         os.replace(tmp, LIB)
+    build_torch(force)
     return LIB
+
+
+def build_torch(force: bool = False) -> str:
+    """Compile the module of csrc/torch_feed_forward.cpp; returns its path."""
+    import torch
+
+    src = os.path.join(CSRC, "torch_feed_forward.cpp")
+    if not (force or _stale(TORCH_LIB, [src, os.path.join(INCLUDE, "pax.h"), torch.__file__])):
+        return TORCH_LIB
+    root = os.path.dirname(torch.__file__)
+    include = [os.path.join(root, "include"), os.path.join(root, "include", "torch", "csrc", "api", "include"),
+               os.path.join(os.path.dirname(os.path.dirname(NVCC)), "include")]
+    tmp = TORCH_LIB + ".tmp"
+    cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared", "-Wall",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", "-I", sysconfig.get_paths()["include"],
+           *(x for d in include for x in ("-isystem", d)), src, "-o", tmp, "-L", os.path.join(root, "lib"),
+           "-ltorch_python", "-ltorch_cpu", "-ltorch_cuda", "-ltorch", "-lc10", "-lc10_cuda", "-L", HERE,
+           "-l:" + os.path.basename(LIB), "-Wl,-rpath,$ORIGIN"]
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    if r.returncode != 0:
+        raise RuntimeError(f"g++ failed for {src}:\n{r.stdout}\n{r.stderr}")
+    os.replace(tmp, TORCH_LIB)
+    return TORCH_LIB
 
 
 if __name__ == "__main__":

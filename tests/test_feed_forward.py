@@ -43,6 +43,14 @@ def test_glu_refuses_types_shapes_and_strides(i):
             pax_b200.glu(*[bad if j == i else t for j, t in enumerate(a)])
 
 
+def test_what_is_not_a_tensor_is_refused():
+    for call in (lambda: pax_b200.glu(None, *glu_args()[1:]), lambda: pax_b200.glu(*glu_args()[:2], [1.0]),
+                 lambda: pax_b200.glu_backward(*back_args(), dX=3), lambda: pax_b200.quantize_rows("x"),
+                 lambda: pax_b200.gemm_i8(h(4, 16, dtype=I8), h(8, 16, dtype=I8), 0.5, h(8, dtype=F32))):
+        with pytest.raises((TypeError, ValueError), match="tensor"):
+            call()
+
+
 def test_glu_refuses_half_of_the_kept_products_and_unknown_activations():
     with pytest.raises(ValueError, match="together"):
         pax_b200.glu(*glu_args(), G=h(4, 8))
