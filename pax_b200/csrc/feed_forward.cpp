@@ -206,24 +206,24 @@ pax_status_t pax_glu_backward_ex(const pax_glu_grad_desc_t* desc, cudaStream_t s
         // The second launch counts as 6 k-blocks, about 2 us.  The choice
         // goes by the shape, not by which gradients are asked for, so that
         // dX has the same bits either way.
-        GluGradProblem rest = p;
+        bool apart = false;
+        GluGradProblem x = p, w = p, both = p;
+        x.dWg = x.dWu = nullptr;
+        w.dX = nullptr;
         if (glu_dx_skinny_ok(p)) {
-            GluGradProblem x = p, w = p, both = p;
-            x.dWg = x.dWu = nullptr;
-            w.dX = nullptr;
-            w.dWg = w.dWu = both.dWg = both.dWu = p.dX;  // asked for; not read here
-            if (!glu_back_tc_ok(x) || glu_dx_skinny_time(p) + glu_back_tc_time(w) + 6.0 < glu_back_tc_time(both)) {
-                st = glu_dx_skinny(p, stream);
-                rest.dX = nullptr;
-            }
+            GluGradProblem asked = w;
+            asked.dWg = asked.dWu = both.dWg = both.dWu = p.dX;  // asked for; not read here
+            apart = !glu_back_tc_ok(x) || glu_dx_skinny_time(p) + glu_back_tc_time(asked) + 6.0 < glu_back_tc_time(both);
         }
-        if (st == PAX_OK && (rest.dX || rest.dWg)) {
-            if (glu_back_tc_ok(rest)) {
-                st = glu_back_tc(rest, stream);
-            } else {
-                if (rest.dX) st = glu_dx_any(rest, stream);
-                if (st == PAX_OK && rest.dWg) st = glu_dw_any(rest, stream);
-            }
+        if (apart) {
+            const bool tc = p.dWg && glu_back_tc_ok(w);
+            if (p.dWg) st = tc ? glu_back_tc(w, stream) : glu_dw_any(w, stream);
+            if (st == PAX_OK) st = glu_dx_skinny(p, tc, stream);
+        } else if (glu_back_tc_ok(p)) {
+            st = glu_back_tc(p, stream);
+        } else {
+            if (p.dX) st = glu_dx_any(p, stream);
+            if (st == PAX_OK && p.dWg) st = glu_dw_any(p, stream);
         }
     }
     return done(st, "pax_glu_backward_ex");

@@ -61,7 +61,7 @@ bool set_wait_limit_ff_tc(unsigned long long ns);
 // the 8-bit product up to 512), with the same kind of expectation.
 bool glu_dx_skinny_ok(const GluGradProblem& p);
 double glu_dx_skinny_time(const GluGradProblem& p);
-pax_status_t glu_dx_skinny(const GluGradProblem& p, cudaStream_t stream);
+pax_status_t glu_dx_skinny(const GluGradProblem& p, bool beside, cudaStream_t stream);
 bool glu_skinny_ok(const GluProblem& p);
 double glu_skinny_time(const GluProblem& p);
 pax_status_t glu_skinny(const GluProblem& p, cudaStream_t stream);

@@ -41,6 +41,7 @@ struct FsParams {
     int M, N, kbs;  // tokens, weight columns, k-blocks
     int rows;       // tokens of a chunk
     int half;       // FS_DX: k-blocks of the first term
+    int beside;     // FS_DX: see glu_dx_skinny
     // FS_GLU; FS_DX: the gradient in H
     __half *H, *G, *U;
     long long ldh, ldg, ldu;
@@ -126,7 +127,7 @@ __global__ void __launch_bounds__(192, R)
     if (warp == 0) {
         // ------------------------------------------------ TMA producer
         if (lane == 0) {
-            pdl_wait();  // the operands may be written by the previous grid
+            if (MODE != FS_DX || !p.beside) pdl_wait();  // the operands may be written by the previous grid
             const int col = tile * TILE;
             int stage = 0, total = 0;
             uint32_t phase = 0;
@@ -193,7 +194,7 @@ __global__ void __launch_bounds__(192, R)
             mbar_wait(done_bar, 0, nullptr);
         }
     } else {
-        pdl_wait();  // outputs and scales may belong to the previous grid
+        if (MODE != FS_DX || !p.beside) pdl_wait();  // outputs and scales may belong to the previous grid
         mbar_wait(done_bar, 0, nullptr);
         __syncwarp();
         tc_fence_after();
@@ -225,6 +226,8 @@ __global__ void __launch_bounds__(192, R)
         tc_fence_after();
         tmem_dealloc<1>(tmem_base, Cfg::TMEM_COLS);
     }
+    // What follows in the stream relies on the grid this one ran beside.
+    if (MODE == FS_DX && p.beside && threadIdx.x == 0) pdl_wait();
     if (*abort_flag) return;
     const float* r = reinterpret_cast<const float*>(smem);
     const int pstart = part_start<TILE>(rank, S), pwidth = part_start<TILE>(rank + 1, S) - pstart;
@@ -492,10 +495,15 @@ double glu_dx_skinny_time(const GluGradProblem& q) {
     return plan_time<FS_DX>(p);
 }
 
-pax_status_t glu_dx_skinny(const GluGradProblem& q, cudaStream_t stream) {
+// beside: the previous launch in the stream is glu_back_tc's for the weight
+// gradients alone, which lets this one start once dG and dU are written.
+// Neither reads what the other writes, so they run side by side where the
+// first leaves SMs free, and this one ends no earlier than the first.
+pax_status_t glu_dx_skinny(const GluGradProblem& q, bool beside, cudaStream_t stream) {
     FsMaps m;
     FsParams p = {};
     dx_params(q, p);
+    p.beside = beside;
     if (!fs_map(&m.w0, q.Wg, false, q.D, q.F, q.ldwg, 64, 128) || !fs_map(&m.w1, q.Wu, false, q.D, q.F, q.ldwu, 64, 128) ||
         !fs_map(&m.x0, q.dG, false, q.M, q.F, q.lddg, 64, (uint32_t)p.rows) ||
         !fs_map(&m.x1, q.dU, false, q.M, q.F, q.lddu, 64, (uint32_t)p.rows))

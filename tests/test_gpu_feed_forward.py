@@ -455,6 +455,25 @@ def test_other_stream_and_calls_at_once(gen, M):
                 assert torch.equal(a, b)
 
 
+@pytest.mark.parametrize("shape", [(40, 264, 520), (130, 768, 2048), (100, 512, 512)])
+def test_backward_passes_in_a_row_with_inputs_that_change(gen, shape):
+    """Passes queued without a pause, the inputs overwritten in place between them: each launch of a pass starts while the one
+    before ends, and none may read what the last pass or the next one writes."""
+    M, D, F = shape
+    sets = [back_inputs(gen, M, D, F) for _ in range(3)]
+    want = [pax_b200.glu_backward(*a) for a in sets]
+    torch.cuda.synchronize()
+    live = [t.clone() for t in sets[0]]
+    wrong = torch.zeros((), device=gen.device, dtype=torch.int64)
+    for i in range(150):
+        for t, new in zip(live, sets[i % 3]):
+            t.copy_(new)
+        got = pax_b200.glu_backward(*live, dG=live[4], dU=live[5])
+        for g, w in zip(got, want[i % 3]):
+            wrong += (g != w).sum()
+    assert wrong.item() == 0
+
+
 CAPTURE_FIRST = """
 import torch, pax_b200
 g = torch.Generator(device="cuda"); g.manual_seed(3)
