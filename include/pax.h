@@ -318,6 +318,10 @@ typedef struct {
     int64_t          M, D, F; /* tokens, model width, feed-forward width   */
     int64_t          ldx, ldwg, ldwu, ldh, ldg, ldu;
     pax_activation_t act;
+    int              w_const; /* Wg and Wu are not written by the kernel launched just
+                               * before on the stream (weights): with at most 64 tokens
+                               * the kernel then starts loading them before that kernel
+                               * has ended.  As PAX_GEMM_B_CONST of pax_gemm_ex. */
 } pax_glu_desc_t;
 pax_status_t pax_glu_ex(const pax_glu_desc_t* desc, cudaStream_t stream);
 
@@ -373,6 +377,7 @@ typedef struct {
     int64_t      M, N, K;
     int64_t      lda, ldb, ldc;
     pax_dtype_t  c_dtype;
+    int          b_const; /* as w_const of pax_glu_desc_t, for B */
 } pax_gemm_i8_desc_t;
 pax_status_t pax_gemm_i8_ex(const pax_gemm_i8_desc_t* desc, cudaStream_t stream);
 

@@ -55,7 +55,7 @@ class GluDesc(ctypes.Structure):
     """pax_glu_desc_t (include/pax.h)."""
     _fields_ = ([(n, ctypes.c_void_p) for n in ("X", "Wg", "Wu", "H", "G", "U")]
                 + [(n, ctypes.c_int64) for n in ("M", "D", "F", "ldx", "ldwg", "ldwu", "ldh", "ldg", "ldu")]
-                + [("act", ctypes.c_int)])
+                + [("act", ctypes.c_int), ("w_const", ctypes.c_int)])
 
 
 class GluGradDesc(ctypes.Structure):
@@ -69,7 +69,8 @@ class GluGradDesc(ctypes.Structure):
 class GemmI8Desc(ctypes.Structure):
     """pax_gemm_i8_desc_t (include/pax.h)."""
     _fields_ = ([(n, ctypes.c_void_p) for n in ("A", "B", "C", "a_scale", "b_scale", "bias")]
-                + [(n, ctypes.c_int64) for n in ("M", "N", "K", "lda", "ldb", "ldc")] + [("c_dtype", ctypes.c_int)])
+                + [(n, ctypes.c_int64) for n in ("M", "N", "K", "lda", "ldb", "ldc")] 
+                + [("c_dtype", ctypes.c_int), ("b_const", ctypes.c_int)])
 
 
 class IpcHandle(ctypes.Structure):

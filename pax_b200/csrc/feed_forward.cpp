@@ -76,6 +76,7 @@ pax_status_t check_glu(const pax_glu_desc_t* d, GluProblem* p) {
     p->M = d->M, p->D = d->D, p->F = d->F;
     p->ldx = d->ldx, p->ldwg = d->ldwg, p->ldwu = d->ldwu, p->ldh = d->ldh, p->ldg = d->ldg, p->ldu = d->ldu;
     p->act = (int)d->act;
+    p->w_const = d->w_const != 0;
     if (p->M == 0 || p->F == 0) return PAX_OK;
     if ((p->G != nullptr) != (p->U != nullptr)) return refuse(PAX_ERR_INVALID, "%s: G and U go together", who);
     if (!matrix_ok(p->X, p->M, p->D, &p->ldx) || !matrix_ok(p->Wg, p->D, p->F, &p->ldwg) ||
@@ -161,6 +162,7 @@ pax_status_t check_i8(const pax_gemm_i8_desc_t* d, I8Problem* p) {
     p->M = d->M, p->N = d->N, p->K = d->K;
     p->lda = d->lda, p->ldb = d->ldb, p->ldc = d->ldc;
     p->c_f16 = d->c_dtype == PAX_DT_F16;
+    p->b_const = d->b_const != 0;
     if (p->M == 0 || p->N == 0) return PAX_OK;
     if (!matrix_ok(p->A, p->M, p->K, &p->lda) || !matrix_ok(p->B, p->N, p->K, &p->ldb) ||
         !matrix_ok_sized(p->C, p->c_f16 ? 2 : 4, p->M, p->N, &p->ldc))

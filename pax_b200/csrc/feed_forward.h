@@ -14,6 +14,7 @@ struct GluProblem {
     long long M, D, F;
     long long ldx, ldwg, ldwu, ldh, ldg, ldu;
     int act;
+    bool w_const;
 };
 
 struct GluGradProblem {
@@ -33,7 +34,7 @@ struct I8Problem {
     const __half* bias;  // may be null
     long long M, N, K;
     long long lda, ldb, ldc;
-    bool c_f16;
+    bool c_f16, b_const;
 };
 
 // feed_forward_any.cu: any layout, any alignment, empty sums.

@@ -42,6 +42,7 @@ struct FsParams {
     int rows;       // tokens of a chunk
     int half;       // FS_DX: k-blocks of the first term
     int beside;     // FS_DX: see glu_dx_skinny
+    int w_const;    // the weights are not written by the previous grid
     // FS_GLU; FS_DX: the gradient in H
     __half *H, *G, *U;
     long long ldh, ldg, ldu;
@@ -127,26 +128,44 @@ __global__ void __launch_bounds__(192, R)
     if (warp == 0) {
         // ------------------------------------------------ TMA producer
         if (lane == 0) {
-            if (MODE != FS_DX || !p.beside) pdl_wait();  // the operands may be written by the previous grid
             const int col = tile * TILE;
             int stage = 0, total = 0;
             uint32_t phase = 0;
-            for (int kb = rank; kb < p.kbs; kb += S) {
-                if (!mbar_wait(empty0 + 8u * stage, phase ^ 1u, abort_flag)) break;
-                const uint32_t fb = full0 + 8u * stage;
-                const uint32_t w = smem_u32(smem + stage * Cfg::STAGE_BYTES);
+            auto load_weights = [&](int kb) {
+                const uint32_t fb = full0 + 8u * stage, w = smem_u32(smem + stage * Cfg::STAGE_BYTES);
                 const int k = kb * Cfg::KB;
-                mbar_arrive_expect_tx(fb, Cfg::W_BYTES + (uint32_t)p.rows * 128u);
                 if constexpr (MODE == FS_GLU) {
                     tma_load_3d(w, &tmW0, fb, col, k, 0);
                     tma_load_3d(w + 8192, &tmW1, fb, col, k, 0);
-                    tma_load_3d(w + Cfg::W_BYTES, &tmX, fb, k, m0, 0);
                 } else {
                     const bool second = MODE == FS_DX && kb >= p.half;
-                    const int kk = second ? k - p.half * Cfg::KB : k;
-                    tma_load_3d(w, second ? &tmW1 : &tmW0, fb, kk, col, 0);
-                    tma_load_3d(w + Cfg::W_BYTES, second ? &tmX1 : &tmX, fb, kk, m0, 0);
+                    tma_load_3d(w, second ? &tmW1 : &tmW0, fb, second ? k - p.half * Cfg::KB : k, col, 0);
                 }
+            };
+            auto load_tokens = [&](int kb) {
+                const uint32_t x = smem_u32(smem + stage * Cfg::STAGE_BYTES) + Cfg::W_BYTES;
+                const bool second = MODE == FS_DX && kb >= p.half;
+                tma_load_3d(x, second ? &tmX1 : &tmX, full0 + 8u * stage,
+                            (second ? kb - p.half : kb) * Cfg::KB, m0, 0);
+            };
+            // Weights that the previous grid does not write: a ring's worth of
+            // them before that grid has ended.  Their bytes are expected
+            // without arriving; a slot is full once the tokens' arrival and
+            // bytes have come too.
+            int early = 0;
+            if (MODE != FS_DX && p.w_const)
+                for (int kb = rank; kb < p.kbs && early < STAGES; kb += S, ++early, ++stage) {
+                    mbar_expect_tx(full0 + 8u * stage, Cfg::W_BYTES);
+                    load_weights(kb);
+                }
+            stage = 0;
+            if (MODE != FS_DX || !p.beside) pdl_wait();  // the operands may be written by the previous grid
+            for (int kb = rank; kb < p.kbs; kb += S) {
+                if (!mbar_wait(empty0 + 8u * stage, phase ^ 1u, abort_flag)) break;
+                const bool have = total < early;
+                mbar_arrive_expect_tx(full0 + 8u * stage, (have ? 0u : Cfg::W_BYTES) + (uint32_t)p.rows * 128u);
+                if (!have) load_weights(kb);
+                load_tokens(kb);
                 ++total;
                 if (++stage == STAGES) {
                     stage = 0;
@@ -468,6 +487,7 @@ pax_status_t glu_skinny(const GluProblem& q, cudaStream_t stream) {
         !fs_map(&m.x0, q.X, false, q.M, q.D, q.ldx, 64, (uint32_t)p.rows))
         return PAX_ERR_CUDA;
     m.x1 = m.x0;
+    p.w_const = q.w_const;
     p.H = q.H, p.G = q.G, p.U = q.U;
     p.ldh = q.ldh, p.ldg = q.ldg, p.ldu = q.ldu;
     p.act = q.act;
@@ -537,6 +557,7 @@ pax_status_t gemm_i8_skinny(const I8Problem& q, cudaStream_t stream) {
         return PAX_ERR_CUDA;
     m.w1 = m.w0;
     m.x1 = m.x0;
+    p.w_const = q.b_const;
     p.C = q.C;
     p.ldc = q.ldc;
     p.sa = q.a_scale, p.sb = q.b_scale, p.bias = q.bias;

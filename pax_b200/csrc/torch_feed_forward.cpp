@@ -176,7 +176,7 @@ PyObject* tuple(std::initializer_list<PyObject*> items) {
 
 PyObject* none() { Py_RETURN_NONE; }
 
-// X, Wg, Wu, activation, save, out, G, U, stream -> H or (H, G, U)
+// X, Wg, Wu, activation, save, out, G, U, stream, w_const -> H or (H, G, U)
 PyObject* glu(PyObject* const* a) {
     const at::Tensor &X = matrix2d(a[0], "X"), &Wg = matrix2d(a[1], "Wg"), &Wu = tensor(a[2], "Wu");
     const int64_t M = X.size(0), D = X.size(1), F = Wg.size(1);
@@ -186,6 +186,7 @@ PyObject* glu(PyObject* const* a) {
     pax_glu_desc_t d = {};
     d.M = M, d.D = D, d.F = F;
     d.act = (pax_activation_t)PyLong_AsLong(a[3]);
+    d.w_const = a[9] == Py_True;
     d.ldx = matrix(X, "X", M, D, at::kHalf, dev);
     d.ldwg = matrix(Wg, "Wg", D, F, at::kHalf, dev);
     d.ldwu = matrix(Wu, "Wu", D, F, at::kHalf, dev);
@@ -281,7 +282,8 @@ PyObject* quantize_rows(PyObject* const* a) {
     return tuple({wrap(a[1], Q), wrap(a[2], scale)});
 }
 
-// A, B, a_scale, b_scale, bias, out, out dtype (0 float32, 1 float16), stream -> C
+// A, B, a_scale, b_scale, bias, out, out dtype (0 float32, 1 float16), stream,
+// b_const -> C
 PyObject* gemm_i8(PyObject* const* a) {
     const at::Tensor &A = matrix2d(a[0], "A"), &B = matrix2d(a[1], "B"), &sa = tensor(a[2], "a_scale"),
                      &sb = tensor(a[3], "b_scale");
@@ -289,6 +291,7 @@ PyObject* gemm_i8(PyObject* const* a) {
     const c10::Device dev = A.device();
     pax_gemm_i8_desc_t d = {};
     d.M = M, d.N = N, d.K = K;
+    d.b_const = a[8] == Py_True;
     d.lda = matrix(A, "A", M, K, at::kChar, dev);
     d.ldb = matrix(B, "B", N, K, at::kChar, dev);
     vector(sa, "a_scale", M, at::kFloat, dev);
@@ -337,8 +340,8 @@ PyObject* entry(PyObject*, PyObject* const* args, Py_ssize_t n) {
 }
 
 #define PAX_ENTRY(f, n) {#f, reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(entry<f, n>)), METH_FASTCALL, nullptr}
-PyMethodDef kMethods[] = {PAX_ENTRY(glu, 9), PAX_ENTRY(glu_backward, 17), PAX_ENTRY(quantize_rows, 4),
-                          PAX_ENTRY(gemm_i8, 8), {nullptr, nullptr, 0, nullptr}};
+PyMethodDef kMethods[] = {PAX_ENTRY(glu, 10), PAX_ENTRY(glu_backward, 17), PAX_ENTRY(quantize_rows, 4),
+                          PAX_ENTRY(gemm_i8, 9), {nullptr, nullptr, 0, nullptr}};
 PyModuleDef kModule = {PyModuleDef_HEAD_INIT, "_feed_forward", nullptr, -1, kMethods, nullptr, nullptr, nullptr, nullptr};
 
 }  // namespace

@@ -54,7 +54,7 @@ def _native():
 
 def glu(X: torch.Tensor, Wg: torch.Tensor, Wu: torch.Tensor, *, activation="silu", save: bool = False,
         out: torch.Tensor | None = None, G: torch.Tensor | None = None, U: torch.Tensor | None = None,
-        stream: torch.cuda.Stream | None = None):
+        stream: torch.cuda.Stream | None = None, w_const: bool = False):
     """H = act(X @ Wg) * (X @ Wu): both projections of a gated feed-forward
     layer, the activation and the product in one kernel.
 
@@ -62,8 +62,11 @@ def glu(X: torch.Tensor, Wg: torch.Tensor, Wu: torch.Tensor, *, activation="silu
     float16 [M, F].  activation is one of silu, gelu_tanh, gelu_erf.  With
     ``save`` (or given G and U) the products X @ Wg and X @ Wu are kept for
     glu_backward, and (H, G, U) is returned instead of H.
+    w_const: Wg and Wu are not written by the kernel launched just before on
+    this stream (weights); with at most 64 tokens the kernel may then start
+    reading them before that kernel ends (as gemm's b_const).
     """
-    return _native().glu(X, Wg, Wu, _activation(activation), bool(save), out, G, U, stream)
+    return _native().glu(X, Wg, Wu, _activation(activation), bool(save), out, G, U, stream, bool(w_const))
 
 
 def glu_backward(dH: torch.Tensor, X: torch.Tensor, Wg: torch.Tensor, Wu: torch.Tensor, G: torch.Tensor, U: torch.Tensor,
@@ -99,14 +102,16 @@ def quantize_rows(X: torch.Tensor, *, out: torch.Tensor | None = None, scale: to
 
 def gemm_i8(A: torch.Tensor, B: torch.Tensor, a_scale: torch.Tensor, b_scale: torch.Tensor, *,
             bias: torch.Tensor | None = None, out: torch.Tensor | None = None,
-            out_dtype: torch.dtype = torch.float16, stream: torch.cuda.Stream | None = None) -> torch.Tensor:
+            out_dtype: torch.dtype = torch.float16, stream: torch.cuda.Stream | None = None,
+            b_const: bool = False) -> torch.Tensor:
     """C = (A @ B.T) * a_scale[:, None] * b_scale[None, :] (+ bias).
 
     A [M, K] and B [N, K] are int8 with unit column stride (what quantize_rows
     gives for tokens and for the weight's output channels), the scales float32
     [M] and [N], bias float16 [N]; C is float16 or float32 [M, N].  The sums
-    are exact 32-bit integers, for K up to 131071.
+    are exact 32-bit integers, for K up to 131071.  b_const: B is not written
+    by the kernel launched just before on this stream, as in gemm.
     """
     if out_dtype not in _DT:
         raise TypeError("out_dtype must be float32 or float16")
-    return _native().gemm_i8(A, B, a_scale, b_scale, bias, out, int(_DT[out_dtype]), stream)
+    return _native().gemm_i8(A, B, a_scale, b_scale, bias, out, int(_DT[out_dtype]), stream, bool(b_const))

@@ -474,6 +474,30 @@ def test_backward_passes_in_a_row_with_inputs_that_change(gen, shape):
     assert wrong.item() == 0
 
 
+@pytest.mark.parametrize("M", [1, 24, 64])
+def test_decoding_chain_with_constant_weights(gen, M):
+    """Layers in a row, each reading what the one before wrote, with their weights marked constant: the same bits as without."""
+    D, F, L = 512, 1032, 6
+    X = randn(gen, M, D)
+    W = [(*weights(gen, D, F), *pax_b200.quantize_rows(randn(gen, D, F, scale=F ** -0.5))) for _ in range(L)]
+
+    def chain(const):
+        x = X
+        for Wg, Wu, Wq, sw in W:
+            H = pax_b200.glu(x, Wg, Wu, w_const=const)
+            Q, s = pax_b200.quantize_rows(H)
+            x = pax_b200.gemm_i8(Q, Wq, s, sw, b_const=const)
+            x = x / x.float().std().clamp_min(1e-3).half()
+            H2 = pax_b200.glu(x, Wg, Wu, w_const=const)  # weights loaded while the first product still runs
+            x = pax_b200.gemm(H2, Wd[:F], b_const=const)
+        return x
+
+    Wd = randn(gen, F, D, scale=F ** -0.5)
+    want = chain(False)
+    for _ in range(20):
+        assert torch.equal(chain(True), want)
+
+
 CAPTURE_FIRST = """
 import torch, pax_b200
 g = torch.Generator(device="cuda"); g.manual_seed(3)
