@@ -26,7 +26,7 @@ INCLUDE = os.path.join(os.path.dirname(HERE), "include")
 NVCC = os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc")
 
 SOURCES = ["gemm_tc_f16.cu", "gemm_tc_f32.cu", "gemm_tc.cu", "gemm_skinny.cu", "gemm_simt.cu", "peer_sync.cu",
-           "feed_forward_tc.cu", "feed_forward_skinny.cu",
+           "feed_forward_tc.cu", "feed_forward_skinny.cu", "feed_forward_split.cu",
            "feed_forward_any.cu", "feed_forward_rows.cu", "feed_forward.cpp", "host_bridge.cpp", "fp16_ops.cpp"]
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 FLAGS = ["-O3", "-std=c++17", "-lineinfo", "-Xcompiler", "-fPIC,-O3", "--expt-relaxed-constexpr", "-I", INCLUDE]

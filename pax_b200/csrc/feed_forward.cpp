@@ -54,6 +54,52 @@ pax_status_t device_ok(const char* who) {
 // in tiles, 256x1024x4096 10.8 and 14.2, but 128x11264x4096 24.0 and 17.5.
 bool chunks_pay(double chunks, double tiles) { return 1.15 * (0.47 * chunks + 5.0) < 0.36 * tiles + 1.0; }
 
+// dX and the weight gradients, from dG and dU.  Both in one launch of tiles,
+// where dX's few and long tiles do not keep it waiting; else dX apart, split
+// along F by clusters of pairs or, for few tokens, on the few-token kernel, and
+// the weight gradients in tiles or split along the tokens.  A second launch
+// counts as 6 k-blocks, about 2 us; a k-block of the few-token kernel, with 64
+// tokens beside it, as 1.3.  The choice goes by the shape, not by which
+// gradients are asked for, so that they have the same bits either way.
+pax_status_t back_products(const GluGradProblem& p, cudaStream_t stream) {
+    if (p.M == 0 || p.D == 0 || p.F == 0) {
+        const pax_status_t st = p.dX ? glu_dx_any(p, stream) : PAX_OK;
+        return st == PAX_OK && p.dWg ? glu_dw_any(p, stream) : st;
+    }
+    GluGradProblem x = p, w = p, both = p;
+    // What both together, dX alone and the weight gradients alone would take;
+    // the pointers stand for "asked for" and are not read.
+    both.dX = x.dX = p.dX ? p.dX : p.dG;
+    both.dWg = both.dWu = w.dWg = w.dWu = p.dWg ? p.dWg : static_cast<void*>(p.dG);
+    x.dWg = x.dWu = nullptr;
+    w.dX = nullptr;
+    const SplitPlan xs = glu_dx_split_plan(p), ws = glu_dw_split_plan(p);
+    const double few = 1.3 * glu_dx_skinny_time(p) + 8.0, wt = glu_back_tc_time(w);
+    const double x_time = few < xs.time ? few : xs.time, w_time = wt < ws.time ? wt : ws.time;
+    const bool apart = x_time + w_time + 6.0 < glu_back_tc_time(both);
+
+    GluGradProblem px = p, pw = p;  // each part as asked for
+    px.dWg = px.dWu = nullptr;
+    pw.dX = nullptr;
+    pax_status_t st = PAX_OK;
+    if (!apart && glu_back_tc_ok(p)) return glu_back_tc(p, stream);
+    // The weight gradients first: dX's few-token kernel can run beside them.
+    bool beside = false;
+    if (p.dWg) {
+        if (!glu_back_tc_ok(pw)) {
+            st = glu_dw_any(pw, stream);
+        } else {
+            beside = true;
+            st = apart && ws.time < wt ? glu_dw_split(pw, ws.S, stream) : glu_back_tc(pw, stream);
+        }
+    }
+    if (st != PAX_OK || !p.dX) return st;
+    const bool tiles_ok = glu_back_tc_ok(px);
+    if (glu_dx_skinny_ok(p) && (!tiles_ok || (apart && few < xs.time))) return glu_dx_skinny(p, beside, stream);
+    if (!tiles_ok) return glu_dx_any(px, stream);
+    return apart ? glu_dx_split(px, xs.S, stream) : glu_back_tc(px, stream);
+}
+
 pax_status_t done(pax_status_t st, const char* who) {
     if (st == PAX_OK) return report_status(PAX_OK, "");
     return refuse(st, "%s: launch failed (%s)", who, pax_status_string(st));
@@ -188,10 +234,17 @@ pax_status_t pax_glu_ex(const pax_glu_desc_t* desc, cudaStream_t stream) {
     if (st != PAX_OK) return st;
     if (p.M == 0 || p.F == 0) return report_status(PAX_OK, "");
     if ((st = device_ok("pax_glu_ex")) != PAX_OK) return st;
-    const bool few = glu_skinny_ok(p), tc = glu_tc_ok(p);
-    st = few && (p.M <= 64 || !tc || chunks_pay(glu_skinny_time(p), glu_tc_time(p))) ? glu_skinny(p, stream)
-         : tc                                                                         ? glu_tc(p, stream)
-                                                                                      : glu_any(p, stream);
+    if (glu_skinny_ok(p) && p.M <= 64) return done(glu_skinny(p, stream), "pax_glu_ex");
+    if (glu_tc_ok(p)) {
+        const double tiles = glu_tc_time(p);
+        const SplitPlan split = glu_split_plan(p);
+        if (glu_skinny_ok(p) && chunks_pay(glu_skinny_time(p), tiles < split.time ? tiles : split.time))
+            st = glu_skinny(p, stream);
+        else
+            st = split.time < tiles ? glu_split(p, split.S, stream) : glu_tc(p, stream);
+    } else {
+        st = glu_skinny_ok(p) ? glu_skinny(p, stream) : glu_any(p, stream);
+    }
     return done(st, "pax_glu_ex");
 }
 
@@ -203,30 +256,7 @@ pax_status_t pax_glu_backward_ex(const pax_glu_grad_desc_t* desc, cudaStream_t s
     if ((st = device_ok("pax_glu_backward_ex")) != PAX_OK) return st;
     st = glu_grad_rows(p, stream);
     if (st == PAX_OK && (p.dX || p.dWg)) {
-        // Few tokens leave dX too few tiles of too many k-blocks for one
-        // launch with the weight gradients: it then runs apart, split along F.
-        // The second launch counts as 6 k-blocks, about 2 us.  The choice
-        // goes by the shape, not by which gradients are asked for, so that
-        // dX has the same bits either way.
-        bool apart = false;
-        GluGradProblem x = p, w = p, both = p;
-        x.dWg = x.dWu = nullptr;
-        w.dX = nullptr;
-        if (glu_dx_skinny_ok(p)) {
-            GluGradProblem asked = w;
-            asked.dWg = asked.dWu = both.dWg = both.dWu = p.dX;  // asked for; not read here
-            apart = !glu_back_tc_ok(x) || glu_dx_skinny_time(p) + glu_back_tc_time(asked) + 6.0 < glu_back_tc_time(both);
-        }
-        if (apart) {
-            const bool tc = p.dWg && glu_back_tc_ok(w);
-            if (p.dWg) st = tc ? glu_back_tc(w, stream) : glu_dw_any(w, stream);
-            if (st == PAX_OK) st = glu_dx_skinny(p, tc, stream);
-        } else if (glu_back_tc_ok(p)) {
-            st = glu_back_tc(p, stream);
-        } else {
-            if (p.dX) st = glu_dx_any(p, stream);
-            if (st == PAX_OK && p.dWg) st = glu_dw_any(p, stream);
-        }
+        st = back_products(p, stream);
     }
     return done(st, "pax_glu_backward_ex");
 }
@@ -253,10 +283,17 @@ pax_status_t pax_gemm_i8_ex(const pax_gemm_i8_desc_t* desc, cudaStream_t stream)
     if (st != PAX_OK) return st;
     if (p.M == 0 || p.N == 0) return report_status(PAX_OK, "");
     if ((st = device_ok("pax_gemm_i8_ex")) != PAX_OK) return st;
-    const bool few = gemm_i8_skinny_ok(p), tc = gemm_i8_tc_ok(p);
-    st = few && (p.M <= 64 || !tc || chunks_pay(gemm_i8_skinny_time(p), gemm_i8_tc_time(p))) ? gemm_i8_skinny(p, stream)
-         : tc                                                                               ? gemm_i8_tc(p, stream)
-                                                                                            : gemm_i8_any(p, stream);
+    if (gemm_i8_skinny_ok(p) && p.M <= 64) return done(gemm_i8_skinny(p, stream), "pax_gemm_i8_ex");
+    if (gemm_i8_tc_ok(p)) {
+        const double tiles = gemm_i8_tc_time(p);
+        const SplitPlan split = gemm_i8_split_plan(p);
+        if (gemm_i8_skinny_ok(p) && chunks_pay(gemm_i8_skinny_time(p), tiles < split.time ? tiles : split.time))
+            st = gemm_i8_skinny(p, stream);
+        else
+            st = split.time < tiles ? gemm_i8_split(p, split.S, stream) : gemm_i8_tc(p, stream);
+    } else {
+        st = gemm_i8_skinny_ok(p) ? gemm_i8_skinny(p, stream) : gemm_i8_any(p, stream);
+    }
     return done(st, "pax_gemm_i8_ex");
 }
 

@@ -58,6 +58,24 @@ pax_status_t gemm_i8_tc(const I8Problem& p, cudaStream_t stream);
 int read_clear_device_error_ff_tc();
 bool set_wait_limit_ff_tc(unsigned long long ns);
 
+// feed_forward_split.cu: few tiles with long sums, S CTA pairs to a tile; for
+// problems that the tiles of feed_forward_tc.cu take.  A plan's time is in the
+// same k-blocks.
+struct SplitPlan {
+    int S = 0;
+    double time = 1e30;
+};
+SplitPlan glu_split_plan(const GluProblem& p);
+pax_status_t glu_split(const GluProblem& p, int S, cudaStream_t stream);
+SplitPlan gemm_i8_split_plan(const I8Problem& p);
+pax_status_t gemm_i8_split(const I8Problem& p, int S, cudaStream_t stream);
+SplitPlan glu_dx_split_plan(const GluGradProblem& p);
+pax_status_t glu_dx_split(const GluGradProblem& p, int S, cudaStream_t stream);
+SplitPlan glu_dw_split_plan(const GluGradProblem& p);
+pax_status_t glu_dw_split(const GluGradProblem& p, int S, cudaStream_t stream);
+int read_clear_device_error_ff_split();
+bool set_wait_limit_ff_split(unsigned long long ns);
+
 // feed_forward_skinny.cu: few tokens, in chunks of at most 64 (the gated and
 // the 8-bit product up to 512), with the same kind of expectation.
 bool glu_dx_skinny_ok(const GluGradProblem& p);

@@ -440,8 +440,9 @@ pax_status_t pax_device_error(void) {
     const int c = read_clear_device_error_peer();
     const int d = read_clear_device_error_ff_tc();
     const int e = read_clear_device_error_ff_skinny();
-    if (a < 0 || b < 0 || c < 0 || d < 0 || e < 0) return set_status(PAX_ERR_CUDA);
-    return set_status((a | b | c | d | e) ? PAX_ERR_TIMEOUT : PAX_OK);
+    const int f = read_clear_device_error_ff_split();
+    if (a < 0 || b < 0 || c < 0 || d < 0 || e < 0 || f < 0) return set_status(PAX_ERR_CUDA);
+    return set_status((a | b | c | d | e | f) ? PAX_ERR_TIMEOUT : PAX_OK);
 }
 
 void pax_shutdown(void) {
@@ -456,7 +457,7 @@ pax_status_t pax_selftest_set_wait_limit(uint64_t ns) {
     if (v < 1000ull) return fail(PAX_ERR_INVALID, "pax_selftest_set_wait_limit: %llu ns is below 1 us", v);
     if (cudaDeviceSynchronize() != cudaSuccess) return fail(PAX_ERR_CUDA, "pax_selftest_set_wait_limit: device error");
     if (!set_wait_limit_tc(v) || !set_wait_limit_skinny(v) || !set_wait_limit_ff_tc(v) ||
-        !set_wait_limit_ff_skinny(v))
+        !set_wait_limit_ff_skinny(v) || !set_wait_limit_ff_split(v))
         return fail(PAX_ERR_CUDA, "pax_selftest_set_wait_limit: copy to the device failed");
     return set_status(PAX_OK);
 }

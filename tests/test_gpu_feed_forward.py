@@ -45,7 +45,7 @@ def weights(g, D, F):
 # tile, ragged tiles on every side, several tiles, and layouts without 16-byte rows
 GLU_SHAPES = [(1, 8, 8), (1, 2048, 1000), (2, 64, 64), (8, 128, 72), (15, 200, 136), (16, 1024, 520), (17, 72, 2056), (33, 512, 64),
               (64, 4096, 256), (65, 264, 328), (100, 1032, 96), (128, 64, 128), (129, 192, 1160), (256, 256, 128), (257, 512, 264),
-              (300, 8, 136), (520, 1096, 640), (1000, 640, 1408),
+              (300, 8, 136), (520, 1096, 640), (1000, 640, 1408), (300, 4096, 136), (513, 2056, 264), (700, 1544, 296),
               (1, 9, 8), (7, 64, 33), (70, 65, 130), (200, 121, 77)]
 
 
@@ -141,6 +141,7 @@ def test_glu_keeps_nan_in_its_row_and_overflows_to_infinity(gen, M):
 
 # ------------------------------------------------------------------ backward
 BACK_SHAPES = [(1, 64, 64), (3, 8, 8), (31, 136, 72), (64, 256, 128), (130, 768, 520), (257, 264, 1032), (512, 512, 256), (700, 1096, 328),
+               (600, 264, 2056), (2500, 136, 264), (1100, 520, 1032), (4100, 72, 72),
                (5, 33, 64), (40, 64, 71), (90, 65, 130)]
 
 
@@ -189,7 +190,7 @@ def test_glu_gradients_agree_with_differences(gen, name):
         assert (got - want).abs() <= bound, (i, got.item(), want.item(), bound.item())
 
 
-@pytest.mark.parametrize("shape", [(130, 72, 136), (40, 33, 65)])
+@pytest.mark.parametrize("shape", [(130, 72, 136), (40, 33, 65), (600, 264, 2056), (2500, 136, 264)])
 def test_glu_backward_parts_accumulation_and_shared_buffers(gen, shape):
     M, D, F = shape
     a = back_inputs(gen, M, D, F)
@@ -290,7 +291,7 @@ def test_quantize_rows_strided_and_empty(gen):
 
 # ------------------------------------------------------------------ 8-bit product
 I8_SHAPES = [(1, 16, 16), (1, 1000, 4096), (3, 128, 128), (16, 264, 144), (17, 8, 2064), (33, 129, 256), (64, 4096, 1024), (65, 300, 400),
-             (128, 256, 128), (130, 333, 1040), (256, 256, 256), (300, 1030, 640), (1000, 515, 272), (1, 5, 7), (20, 33, 30), (90, 70, 129),
+             (128, 256, 128), (130, 333, 1040), (256, 256, 256), (300, 1030, 640), (1000, 515, 272), (500, 300, 4112), (300, 515, 8192), (1, 5, 7), (20, 33, 30), (90, 70, 129),
              (2, 64, 32768)]
 
 
