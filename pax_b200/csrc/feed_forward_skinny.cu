@@ -376,7 +376,7 @@ pax_status_t launch_split(const FsMaps& m, const FsParams& p, long long tiles, i
 // Measured against it at D = 4096, with a fixed 2 us on top: 74 tiles unsplit,
 // R = 2, 22.0 us (model 23); 176 tiles, R = 2, 35.0 (35), in pairs at R = 3,
 // 31.0 (28); 350 tiles, R = 3, 57.9 (55).  Over 19 shapes of 1 to 64 tokens
-// the choice is the best of 14 tried by hand, or within 5 % of it.
+// the choice is the best of 14 tried by hand, or within 6 % of it.
 double fs_wave_time(long long n, double kb, int R, int sms) {
     const double cap = R == 2 ? 1.0 : 0.85;
     const long long a = n / sms, rem = n % sms;
@@ -404,7 +404,9 @@ FsPlan fs_plan(const FsParams& p) {
     // two per SM 10.8); or unsplit in several waves.
     for (int r = 2; r <= 3; ++r)
         for (int s = 1; s <= kMaxSplit; ++s) {
-            if (s > 1 && (tiles * s > (long long)r * sms || p.kbs < 2 * s)) break;
+            // CTAs that share an SM with others take four k-blocks at least
+            // (16x1024x2816 with two: 6.9 us, with four 5.7).
+            if (s > 1 && (tiles * s > (long long)r * sms || p.kbs < (tiles * s > sms ? 4 : 2) * s)) break;
             const long long n = r == 2 ? fs_clusters<MODE, MP, 2>(dev, s) : fs_clusters<MODE, MP, 3>(dev, s);
             if (n <= 0 || (s > 1 && tiles > n)) continue;
             const long long waves = (tiles - 1) / n;  // before the last one
