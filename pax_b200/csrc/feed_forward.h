@@ -37,6 +37,16 @@ struct I8Problem {
     bool c_f16, b_const;
 };
 
+// Rows that TMA can read: base and pitch of whole 16-byte units.
+inline bool rows16(const void* p, long long ld, int elem) {
+    return (reinterpret_cast<uintptr_t>(p) & 15u) == 0 && (ld * elem) % 16 == 0;
+}
+// Output rows that it may write: a store covers whole 16-byte units, so that a
+// width that ends inside one would write beyond it.
+inline bool out16(const void* p, long long cols, long long ld, int elem) {
+    return rows16(p, ld, elem) && (cols * elem) % 16 == 0;
+}
+
 // feed_forward_any.cu: any layout, any alignment, empty sums.
 pax_status_t glu_any(const GluProblem& p, cudaStream_t stream);
 pax_status_t glu_dx_any(const GluGradProblem& p, cudaStream_t stream);

@@ -94,10 +94,6 @@ __global__ void __launch_bounds__(kGradThreads) glu_grad_kernel(const GluGradPro
     }
 }
 
-bool row16(const void* p, long long ld, int elem) {
-    return (reinterpret_cast<uintptr_t>(p) & 15u) == 0 && (ld * elem) % 16 == 0;
-}
-
 // A launch that may start while the previous kernel in the stream ends.
 template <typename... Params, typename... Args>
 pax_status_t launch_rows(void (*kern)(Params...), long long grid, int threads, cudaStream_t stream, Args... args) {
@@ -127,8 +123,8 @@ pax_status_t launch_grad_index(const GluGradProblem& p, cudaStream_t stream) {
 
 template <int ACT>
 pax_status_t launch_grad(const GluGradProblem& p, cudaStream_t stream) {
-    const bool vec = p.F % 8 == 0 && row16(p.dH, p.lddh, 2) && row16(p.G, p.ldg, 2) && row16(p.U, p.ldu, 2) &&
-                     row16(p.dG, p.lddg, 2) && row16(p.dU, p.lddu, 2);
+    const bool vec = p.F % 8 == 0 && rows16(p.dH, p.lddh, 2) && rows16(p.G, p.ldg, 2) && rows16(p.U, p.ldu, 2) &&
+                     rows16(p.dG, p.lddg, 2) && rows16(p.dU, p.lddu, 2);
     return vec ? launch_grad_index<ACT, true>(p, stream) : launch_grad_index<ACT, false>(p, stream);
 }
 
@@ -274,7 +270,7 @@ pax_status_t glu_grad_rows(const GluGradProblem& p, cudaStream_t stream) {
 pax_status_t quantize_rows(const __half* X, long long ldx, int8_t* Q, long long ldq, float* scale, long long M,
                            long long K, cudaStream_t stream) {
     if (M == 0) return PAX_OK;
-    const bool vec = K % 8 == 0 && row16(X, ldx, 2) && (reinterpret_cast<uintptr_t>(Q) & 7u) == 0 && ldq % 8 == 0;
+    const bool vec = K % 8 == 0 && rows16(X, ldx, 2) && (reinterpret_cast<uintptr_t>(Q) & 7u) == 0 && ldq % 8 == 0;
     if (!vec) return launch_rows(quantize_rows_twice_kernel<false>, M, 256, stream, X, ldx, Q, ldq, scale, K);
     if (K > 8 * 256 * 8) return launch_rows(quantize_rows_twice_kernel<true>, M, 256, stream, X, ldx, Q, ldq, scale, K);
     const int units = (int)(K / 8);

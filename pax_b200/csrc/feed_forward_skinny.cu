@@ -284,19 +284,6 @@ __global__ void __launch_bounds__(192, R)
 }
 
 // ------------------------------------------------------------------ host
-bool fs_map(CUtensorMap* m, const void* base, bool i8, long long rows, long long cols, long long ld, uint32_t box_cols,
-            uint32_t box_rows) {
-    auto enc = tensor_map_encoder();
-    if (!enc) return false;
-    const uint64_t pitch = (uint64_t)ld * (i8 ? 1 : 2);
-    cuuint64_t dims[3] = {(cuuint64_t)cols, (cuuint64_t)rows, 1};
-    cuuint64_t strides[2] = {pitch, (pitch * (uint64_t)rows + 15) & ~uint64_t(15)};
-    cuuint32_t box[3] = {box_cols, box_rows, 1}, estr[3] = {1, 1, 1};
-    return enc(m, i8 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, const_cast<void*>(base),
-               dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
-               CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
-}
-
 constexpr int kMaxSplit = 8;
 
 
@@ -455,10 +442,6 @@ int chunk_rows(long long M) {
     return (int)((M + chunks - 1) / chunks);
 }
 
-bool rows16(const void* p, long long ld, int elem) {
-    return (reinterpret_cast<uintptr_t>(p) & 15u) == 0 && (ld * elem) % 16 == 0;
-}
-
 }  // namespace
 
 // More tokens than this never read the weights again for another chunk.
@@ -485,8 +468,8 @@ pax_status_t glu_skinny(const GluProblem& q, cudaStream_t stream) {
     FsMaps m;
     FsParams p = {};
     glu_params(q, p);
-    if (!fs_map(&m.w0, q.Wg, false, q.D, q.F, q.ldwg, 64, 64) || !fs_map(&m.w1, q.Wu, false, q.D, q.F, q.ldwu, 64, 64) ||
-        !fs_map(&m.x0, q.X, false, q.M, q.D, q.ldx, 64, (uint32_t)p.rows))
+    if (!matrix_map(&m.w0, q.Wg, kF16, 2, q.D, q.F, q.ldwg, 64, 64) || !matrix_map(&m.w1, q.Wu, kF16, 2, q.D, q.F, q.ldwu, 64, 64) ||
+        !matrix_map(&m.x0, q.X, kF16, 2, q.M, q.D, q.ldx, 64, (uint32_t)p.rows))
         return PAX_ERR_CUDA;
     m.x1 = m.x0;
     p.w_const = q.w_const;
@@ -526,9 +509,9 @@ pax_status_t glu_dx_skinny(const GluGradProblem& q, bool beside, cudaStream_t st
     FsParams p = {};
     dx_params(q, p);
     p.beside = beside;
-    if (!fs_map(&m.w0, q.Wg, false, q.D, q.F, q.ldwg, 64, 128) || !fs_map(&m.w1, q.Wu, false, q.D, q.F, q.ldwu, 64, 128) ||
-        !fs_map(&m.x0, q.dG, false, q.M, q.F, q.lddg, 64, (uint32_t)p.rows) ||
-        !fs_map(&m.x1, q.dU, false, q.M, q.F, q.lddu, 64, (uint32_t)p.rows))
+    if (!matrix_map(&m.w0, q.Wg, kF16, 2, q.D, q.F, q.ldwg, 64, 128) || !matrix_map(&m.w1, q.Wu, kF16, 2, q.D, q.F, q.ldwu, 64, 128) ||
+        !matrix_map(&m.x0, q.dG, kF16, 2, q.M, q.F, q.lddg, 64, (uint32_t)p.rows) ||
+        !matrix_map(&m.x1, q.dU, kF16, 2, q.M, q.F, q.lddu, 64, (uint32_t)p.rows))
         return PAX_ERR_CUDA;
     return launch_tokens<FS_DX>(m, p, stream);
 }
@@ -554,8 +537,8 @@ pax_status_t gemm_i8_skinny(const I8Problem& q, cudaStream_t stream) {
     FsMaps m;
     FsParams p = {};
     i8_params(q, p);
-    if (!fs_map(&m.w0, q.B, true, q.N, q.K, q.ldb, 128, 128) ||
-        !fs_map(&m.x0, q.A, true, q.M, q.K, q.lda, 128, (uint32_t)p.rows))
+    if (!matrix_map(&m.w0, q.B, kU8, 1, q.N, q.K, q.ldb, 128, 128) ||
+        !matrix_map(&m.x0, q.A, kU8, 1, q.M, q.K, q.lda, 128, (uint32_t)p.rows))
         return PAX_ERR_CUDA;
     m.w1 = m.w0;
     m.x1 = m.x0;

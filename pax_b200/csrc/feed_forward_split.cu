@@ -428,9 +428,6 @@ pax_status_t launch_split(const SpMaps& maps, const SpParams& p, long long tiles
     return cudaLaunchKernelEx(&cfg, ff_split_kernel<MODE, ACT, OutT>, maps, p) == cudaSuccess ? PAX_OK : PAX_ERR_CUDA;
 }
 
-constexpr CUtensorMapDataType kF16 = CU_TENSOR_MAP_DATA_TYPE_FLOAT16, kF32 = CU_TENSOR_MAP_DATA_TYPE_FLOAT32,
-                              kU8 = CU_TENSOR_MAP_DATA_TYPE_UINT8;
-
 }  // namespace
 
 SplitPlan glu_split_plan(const GluProblem& q) { return plan_split((long long)up(q.M, 256) * up(q.F, 128), up(q.D, 64)); }
@@ -438,11 +435,11 @@ SplitPlan glu_split_plan(const GluProblem& q) { return plan_split((long long)up(
 pax_status_t glu_split(const GluProblem& q, int S, cudaStream_t stream) {
     SpMaps maps;
     CUtensorMap* m = maps.m;
-    if (!ff_map(&m[0], q.X, kF16, 2, q.M, q.D, q.ldx, 64, 128) || !ff_map(&m[1], q.Wg, kF16, 2, q.D, q.F, q.ldwg, 64, 64) ||
-        !ff_map(&m[2], q.Wu, kF16, 2, q.D, q.F, q.ldwu, 64, 64) || !ff_map(&m[3], q.H, kF16, 2, q.M, q.F, q.ldh, 64, 32))
+    if (!matrix_map(&m[0], q.X, kF16, 2, q.M, q.D, q.ldx, 64, 128) || !matrix_map(&m[1], q.Wg, kF16, 2, q.D, q.F, q.ldwg, 64, 64) ||
+        !matrix_map(&m[2], q.Wu, kF16, 2, q.D, q.F, q.ldwu, 64, 64) || !matrix_map(&m[3], q.H, kF16, 2, q.M, q.F, q.ldh, 64, 32))
         return PAX_ERR_CUDA;
     m[4] = m[5] = m[3];
-    if (q.G && (!ff_map(&m[4], q.G, kF16, 2, q.M, q.F, q.ldg, 64, 32) || !ff_map(&m[5], q.U, kF16, 2, q.M, q.F, q.ldu, 64, 32)))
+    if (q.G && (!matrix_map(&m[4], q.G, kF16, 2, q.M, q.F, q.ldg, 64, 32) || !matrix_map(&m[5], q.U, kF16, 2, q.M, q.F, q.ldu, 64, 32)))
         return PAX_ERR_CUDA;
     SpParams p = {};
     p.M = (int)q.M, p.N = (int)q.F;
@@ -464,11 +461,11 @@ pax_status_t gemm_i8_split(const I8Problem& q, int S, cudaStream_t stream) {
     CUtensorMap* m = maps.m;
     const int ce = q.c_f16 ? 2 : 4;
     SpParams p = {};
-    p.c_tma = (reinterpret_cast<uintptr_t>(q.C) & 15u) == 0 && (q.ldc * ce) % 16 == 0 && (q.N * ce) % 16 == 0;
-    if (!ff_map(&m[0], q.A, kU8, 1, q.M, q.K, q.lda, 128, 128) || !ff_map(&m[1], q.B, kU8, 1, q.N, q.K, q.ldb, 128, 128))
+    p.c_tma = out16(q.C, q.N, q.ldc, ce);
+    if (!matrix_map(&m[0], q.A, kU8, 1, q.M, q.K, q.lda, 128, 128) || !matrix_map(&m[1], q.B, kU8, 1, q.N, q.K, q.ldb, 128, 128))
         return PAX_ERR_CUDA;
     m[2] = m[3] = m[4] = m[5] = m[0];
-    if (p.c_tma && !ff_map(&m[2], q.C, q.c_f16 ? kF16 : kF32, ce, q.M, q.N, q.ldc, 128 / ce, 32)) return PAX_ERR_CUDA;
+    if (p.c_tma && !matrix_map(&m[2], q.C, q.c_f16 ? kF16 : kF32, ce, q.M, q.N, q.ldc, 128 / ce, 32)) return PAX_ERR_CUDA;
     p.M = (int)q.M, p.N = (int)q.N;
     p.tiles_m = up(q.M, 256), p.tiles_n = up(q.N, 256);
     p.kbs = up(q.K, 128);
@@ -486,9 +483,9 @@ SplitPlan glu_dx_split_plan(const GluGradProblem& q) {
 pax_status_t glu_dx_split(const GluGradProblem& q, int S, cudaStream_t stream) {
     SpMaps maps;
     CUtensorMap* m = maps.m;
-    if (!ff_map(&m[0], q.dG, kF16, 2, q.M, q.F, q.lddg, 64, 128) || !ff_map(&m[1], q.dU, kF16, 2, q.M, q.F, q.lddu, 64, 128) ||
-        !ff_map(&m[2], q.Wg, kF16, 2, q.D, q.F, q.ldwg, 64, 128) || !ff_map(&m[3], q.Wu, kF16, 2, q.D, q.F, q.ldwu, 64, 128) ||
-        !ff_map(&m[4], q.dX, kF16, 2, q.M, q.D, q.lddx, 64, 32))
+    if (!matrix_map(&m[0], q.dG, kF16, 2, q.M, q.F, q.lddg, 64, 128) || !matrix_map(&m[1], q.dU, kF16, 2, q.M, q.F, q.lddu, 64, 128) ||
+        !matrix_map(&m[2], q.Wg, kF16, 2, q.D, q.F, q.ldwg, 64, 128) || !matrix_map(&m[3], q.Wu, kF16, 2, q.D, q.F, q.ldwu, 64, 128) ||
+        !matrix_map(&m[4], q.dX, kF16, 2, q.M, q.D, q.lddx, 64, 32))
         return PAX_ERR_CUDA;
     m[5] = m[4];
     SpParams p = {};
@@ -507,10 +504,10 @@ pax_status_t glu_dw_split(const GluGradProblem& q, int S, cudaStream_t stream) {
     CUtensorMap* m = maps.m;
     const int we = q.dw_f16 ? 2 : 4;
     const CUtensorMapDataType wt = q.dw_f16 ? kF16 : kF32;
-    if (!ff_map(&m[0], q.X, kF16, 2, q.M, q.D, q.ldx, 64, 64) || !ff_map(&m[1], q.dG, kF16, 2, q.M, q.F, q.lddg, 64, 64) ||
-        !ff_map(&m[2], q.dU, kF16, 2, q.M, q.F, q.lddu, 64, 64) ||
-        !ff_map(&m[3], q.dWg, wt, we, q.D, q.F, q.lddwg, 128 / we, 32) ||
-        !ff_map(&m[4], q.dWu, wt, we, q.D, q.F, q.lddwu, 128 / we, 32))
+    if (!matrix_map(&m[0], q.X, kF16, 2, q.M, q.D, q.ldx, 64, 64) || !matrix_map(&m[1], q.dG, kF16, 2, q.M, q.F, q.lddg, 64, 64) ||
+        !matrix_map(&m[2], q.dU, kF16, 2, q.M, q.F, q.lddu, 64, 64) ||
+        !matrix_map(&m[3], q.dWg, wt, we, q.D, q.F, q.lddwg, 128 / we, 32) ||
+        !matrix_map(&m[4], q.dWu, wt, we, q.D, q.F, q.lddwu, 128 / we, 32))
         return PAX_ERR_CUDA;
     m[5] = m[4];
     SpParams p = {};

@@ -6,19 +6,6 @@ namespace pax {
 
 namespace {
 
-constexpr CUtensorMapDataType kF16 = CU_TENSOR_MAP_DATA_TYPE_FLOAT16, kF32 = CU_TENSOR_MAP_DATA_TYPE_FLOAT32,
-                              kU8 = CU_TENSOR_MAP_DATA_TYPE_UINT8;
-
-bool rows16(const void* p, long long ld, int elem) {
-    return (reinterpret_cast<uintptr_t>(p) & 15u) == 0 && (ld * elem) % 16 == 0;
-}
-
-// Output rows that TMA stores may write: a store covers whole 16-byte units,
-// so that a width that ends inside one would write beyond it.
-bool out16(const void* p, long long cols, long long ld, int elem) {
-    return rows16(p, ld, elem) && (cols * elem) % 16 == 0;
-}
-
 int up(long long a, int b) { return (int)((a + b - 1) / b); }
 
 // Tiles run in column-major groups of this many tile rows (as in
@@ -156,13 +143,13 @@ pax_status_t glu_tc(const GluProblem& q, cudaStream_t stream) {
     FfMaps maps;
     FfParams p = {};
     CUtensorMap* m = maps.m;
-    bool ok = ff_map(&m[MG_X], q.X, kF16, 2, q.M, q.D, q.ldx, 64, 128) &&
-              ff_map(&m[MG_WG], q.Wg, kF16, 2, q.D, q.F, q.ldwg, 64, 64) &&
-              ff_map(&m[MG_WU], q.Wu, kF16, 2, q.D, q.F, q.ldwu, 64, 64) &&
-              ff_map(&m[MG_H], q.H, kF16, 2, q.M, q.F, q.ldh, 64, 32);
+    bool ok = matrix_map(&m[MG_X], q.X, kF16, 2, q.M, q.D, q.ldx, 64, 128) &&
+              matrix_map(&m[MG_WG], q.Wg, kF16, 2, q.D, q.F, q.ldwg, 64, 64) &&
+              matrix_map(&m[MG_WU], q.Wu, kF16, 2, q.D, q.F, q.ldwu, 64, 64) &&
+              matrix_map(&m[MG_H], q.H, kF16, 2, q.M, q.F, q.ldh, 64, 32);
     if (ok && q.G)
-        ok = ff_map(&m[MG_G], q.G, kF16, 2, q.M, q.F, q.ldg, 64, 32) &&
-             ff_map(&m[MG_U], q.U, kF16, 2, q.M, q.F, q.ldu, 64, 32);
+        ok = matrix_map(&m[MG_G], q.G, kF16, 2, q.M, q.F, q.ldg, 64, 32) &&
+             matrix_map(&m[MG_U], q.U, kF16, 2, q.M, q.F, q.ldu, 64, 32);
     if (!ok) return PAX_ERR_CUDA;
     for (int i = q.G ? MG_U + 1 : MG_H + 1; i < 10; ++i) m[i] = m[MG_X];
     p.M = (int)q.M;
@@ -216,17 +203,17 @@ pax_status_t glu_back_tc(const GluGradProblem& q, cudaStream_t stream) {
     const int we = q.dw_f16 ? 2 : 4;
     bool ok = true;
     if (q.dX)
-        ok = ff_map(&m[MB_DGK], q.dG, kF16, 2, q.M, q.F, q.lddg, 64, 128) &&
-             ff_map(&m[MB_DUK], q.dU, kF16, 2, q.M, q.F, q.lddu, 64, 128) &&
-             ff_map(&m[MB_WGK], q.Wg, kF16, 2, q.D, q.F, q.ldwg, 64, 128) &&
-             ff_map(&m[MB_WUK], q.Wu, kF16, 2, q.D, q.F, q.ldwu, 64, 128) &&
-             ff_map(&m[MB_DX], q.dX, kF16, 2, q.M, q.D, q.lddx, 64, 32);
+        ok = matrix_map(&m[MB_DGK], q.dG, kF16, 2, q.M, q.F, q.lddg, 64, 128) &&
+             matrix_map(&m[MB_DUK], q.dU, kF16, 2, q.M, q.F, q.lddu, 64, 128) &&
+             matrix_map(&m[MB_WGK], q.Wg, kF16, 2, q.D, q.F, q.ldwg, 64, 128) &&
+             matrix_map(&m[MB_WUK], q.Wu, kF16, 2, q.D, q.F, q.ldwu, 64, 128) &&
+             matrix_map(&m[MB_DX], q.dX, kF16, 2, q.M, q.D, q.lddx, 64, 32);
     if (ok && q.dWg)
-        ok = ff_map(&m[MB_DGN], q.dG, kF16, 2, q.M, q.F, q.lddg, 64, 64) &&
-             ff_map(&m[MB_DUN], q.dU, kF16, 2, q.M, q.F, q.lddu, 64, 64) &&
-             ff_map(&m[MB_XN], q.X, kF16, 2, q.M, q.D, q.ldx, 64, 64) &&
-             ff_map(&m[MB_DWG], q.dWg, wt, we, q.D, q.F, q.lddwg, 128 / we, 32) &&
-             ff_map(&m[MB_DWU], q.dWu, wt, we, q.D, q.F, q.lddwu, 128 / we, 32);
+        ok = matrix_map(&m[MB_DGN], q.dG, kF16, 2, q.M, q.F, q.lddg, 64, 64) &&
+             matrix_map(&m[MB_DUN], q.dU, kF16, 2, q.M, q.F, q.lddu, 64, 64) &&
+             matrix_map(&m[MB_XN], q.X, kF16, 2, q.M, q.D, q.ldx, 64, 64) &&
+             matrix_map(&m[MB_DWG], q.dWg, wt, we, q.D, q.F, q.lddwg, 128 / we, 32) &&
+             matrix_map(&m[MB_DWU], q.dWu, wt, we, q.D, q.F, q.lddwu, 128 / we, 32);
     if (!ok) return PAX_ERR_CUDA;
     // Maps of what is not computed are never used.
     if (!q.dX) m[MB_DGK] = m[MB_DUK] = m[MB_WGK] = m[MB_WUK] = m[MB_DX] = m[MB_XN];
@@ -250,13 +237,13 @@ pax_status_t gemm_i8_tc(const I8Problem& q, cudaStream_t stream) {
     FfParams p = {};
     CUtensorMap* m = maps.m;
     const int ce = q.c_f16 ? 2 : 4;
-    bool ok = ff_map(&m[MI_A], q.A, kU8, 1, q.M, q.K, q.lda, 128, 128) &&
-              ff_map(&m[MI_B], q.B, kU8, 1, q.N, q.K, q.ldb, 128, 128) &&
-              ff_map(&m[MI_B2], q.B, kU8, 1, q.N, q.K, q.ldb, 128, 64) &&
-              ff_map(&m[MI_B4], q.B, kU8, 1, q.N, q.K, q.ldb, 128, 32);
+    bool ok = matrix_map(&m[MI_A], q.A, kU8, 1, q.M, q.K, q.lda, 128, 128) &&
+              matrix_map(&m[MI_B], q.B, kU8, 1, q.N, q.K, q.ldb, 128, 128) &&
+              matrix_map(&m[MI_B2], q.B, kU8, 1, q.N, q.K, q.ldb, 128, 64) &&
+              matrix_map(&m[MI_B4], q.B, kU8, 1, q.N, q.K, q.ldb, 128, 32);
     p.c_tma = out16(q.C, q.N, q.ldc, ce);
     m[MI_C] = m[MI_A];
-    if (ok && p.c_tma) ok = ff_map(&m[MI_C], q.C, q.c_f16 ? kF16 : kF32, ce, q.M, q.N, q.ldc, 128 / ce, 32);
+    if (ok && p.c_tma) ok = matrix_map(&m[MI_C], q.C, q.c_f16 ? kF16 : kF32, ce, q.M, q.N, q.ldc, 128 / ce, 32);
     if (!ok) return PAX_ERR_CUDA;
     for (int i = MI_C + 1; i < 10; ++i) m[i] = m[MI_A];
     p.M = (int)q.M;

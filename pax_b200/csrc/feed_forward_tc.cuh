@@ -608,21 +608,6 @@ __global__ void __launch_bounds__(FfCfg<MODE, W>::THREADS, 1)
 // Host side
 // ======================================================================
 
-// Map of a row-major matrix, rows x cols elements, ld elements between rows;
-// box of box_cols x box_rows, 128B swizzle.
-inline bool ff_map(CUtensorMap* m, const void* base, CUtensorMapDataType dt, int elem, long long rows, long long cols,
-                   long long ld, uint32_t box_cols, uint32_t box_rows) {
-    auto enc = tensor_map_encoder();
-    if (!enc) return false;
-    const uint64_t pitch = (uint64_t)ld * elem;
-    cuuint64_t dims[3] = {(cuuint64_t)cols, (cuuint64_t)rows, 1};
-    cuuint64_t strides[2] = {pitch, (pitch * (uint64_t)rows + 15) & ~uint64_t(15)};
-    cuuint32_t box[3] = {box_cols, box_rows, 1}, estr[3] = {1, 1, 1};
-    return enc(m, dt, 3, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
-               CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
-}
-
 // Allow the kernel its shared memory on the current device: per device and
 // context, and cheap to repeat.
 template <int MODE, int ACT, typename OutT, int W>
