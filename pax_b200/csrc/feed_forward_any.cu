@@ -13,7 +13,7 @@
 // memory, the next step's into registers while this one multiplies, and lie
 // in shared memory the way they were read.  Bound by the number of those
 // loads, 32 a thread for 32 k: glu 4096x4095x4097 takes 2.17 ms (127 TF/s), its
-// backward pass 4.62 ms, the 8-bit product of that shape 1.01 ms; with few
+// backward pass 4.62 ms, the 8-bit product of that shape 1.17 ms; with few
 // tokens each step waits for its loads (glu 7x1001x2001 37 us).
 #include "activation.cuh"
 #include "feed_forward.h"
@@ -44,12 +44,19 @@ struct AnyParams {
 constexpr int kThreads = 256, kStep = 32;  // k of a step
 
 // X outer positions x kStep k of one operand: in registers, then in shared
-// memory as [outer][k] (RED: k is contiguous in memory) or [k][outer].
+// memory as [outer][k] (RED: k is contiguous in memory) or [k][outer].  A
+// fragment has to start on 32 bytes, so 8-bit k lie in two slabs of 16, 48
+// bytes from row to row.
 template <typename T, int X, bool RED>
 struct AnyTile {
+    static_assert(RED || sizeof(T) == 2, "8-bit operands have k contiguous");
     static constexpr int PER = X * kStep / kThreads;
-    static constexpr int LD = RED ? kStep + (sizeof(T) == 1 ? 16 : 8) : X + 8;  // whole 16-byte units
-    static constexpr int ELEMS = RED ? X * LD : kStep * LD;
+    static constexpr int LD = sizeof(T) == 1 ? 48 : RED ? kStep + 8 : X + 8;
+    static constexpr int ELEMS = sizeof(T) == 1 ? 2 * X * LD : RED ? X * LD : kStep * LD;
+    // Where outer position x, k r lies.
+    static __device__ __forceinline__ int at(int x, int r) {
+        return sizeof(T) == 1 ? ((r >> 4) * X + x) * LD + (r & 15) : RED ? x * LD + r : r * LD + x;
+    }
     T v[PER];
 
     __device__ __forceinline__ void load(const AnyOperand& o, long long o0, long long omax, long long r0, long long rmax) {
@@ -80,9 +87,9 @@ struct AnyTile {
 #pragma unroll
         for (int j = 0; j < PER; ++j) {
             if constexpr (RED)
-                s[(t / kStep + j * (kThreads / kStep)) * LD + t % kStep] = v[j];
+                s[at(t / kStep + j * (kThreads / kStep), t % kStep)] = v[j];
             else
-                s[(t / X + j * (kThreads / X)) * LD + t % X] = v[j];
+                s[at(t % X, t / X + j * (kThreads / X))] = v[j];
         }
     }
 };
@@ -136,15 +143,13 @@ __global__ void __launch_bounds__(kThreads) feed_forward_any_kernel(const AnyPar
             wmma::fragment<wmma::matrix_a, 16, 16, 16, T, LayoutA> fa[2];
 #pragma unroll
             for (int i = 0; i < 2; ++i)
-                wmma::load_matrix_sync(fa[i], A_RED ? sA + (wm + 16 * i) * TileA::LD + kk : sA + kk * TileA::LD + wm + 16 * i,
-                                       TileA::LD);
+                wmma::load_matrix_sync(fa[i], sA + TileA::at(wm + 16 * i, kk), TileA::LD);
 #pragma unroll
             for (int c = 0; c < NACC; ++c)
 #pragma unroll
                 for (int j = 0; j < FN; ++j) {
                     wmma::fragment<wmma::matrix_b, 16, 16, 16, T, LayoutB> fb;
-                    wmma::load_matrix_sync(
-                        fb, B_RED ? sB[c] + (wn + 16 * j) * TileB::LD + kk : sB[c] + kk * TileB::LD + wn + 16 * j, TileB::LD);
+                    wmma::load_matrix_sync(fb, sB[c] + TileB::at(wn + 16 * j, kk), TileB::LD);
 #pragma unroll
                     for (int i = 0; i < 2; ++i) wmma::mma_sync(acc[c][i][j], fa[i], fb, acc[c][i][j]);
                 }

@@ -353,6 +353,39 @@ def test_gemm_i8_empty_sum_and_scales_that_are_not_finite(gen, M):
     assert C[1].isnan().all() and (C[0, 5] == 0) and C[2].isfinite().all()
 
 
+# ------------------------------------------------------------------ large
+@pytest.mark.slow
+@pytest.mark.parametrize("extra", [0, 1])
+def test_offsets_beyond_32_bits(gen, extra):
+    """More than 2^31 elements a matrix, in aligned rows and in rows that are not: the last rows are where a 32-bit offset
+    would go astray."""
+    M, F, D = 66000, 32768 + extra, 64
+    last = slice(M - 130, M)
+    X, (Wg, Wu) = randn(gen, M, D), weights(gen, D, F)
+    H, G, U = pax_b200.glu(X, Wg, Wu, save=True)
+    ref = glu(X[last], Wg, Wu, "silu")
+    for what, t in (("H", H), ("G", G), ("U", U)):
+        close(t[last], ref[what], what)
+    dG, dU = torch.empty_like(G), torch.empty_like(G)
+    dX, _, _ = pax_b200.glu_backward(H, X, Wg, Wu, G, U, dG=dG, dU=dU, need_dW=False)
+    ref = glu_grad(H[last], X[last], Wg, Wu, G[last], U[last], "silu")
+    for what, t in (("dX", dX), ("dG", dG), ("dU", dU)):
+        close(t[last], ref[what], what)
+    del dG, dU, U, G
+    Q, s = pax_b200.quantize_rows(H)
+    assert torch.equal(Q[last], quantize(H[last])[0])
+    del H
+    # the same for the 8-bit product's output and for its operand
+    A, B = codes(gen, M, 80), codes(gen, F, 80)
+    sa, sb = torch.rand(M, generator=gen, device=gen.device) * 1e-2, torch.rand(F, generator=gen, device=gen.device) * 1e-2
+    C = pax_b200.gemm_i8(A, B, sa, sb)
+    close(C[last], gemm_i8(A[last], B, sa[last], sb, None, True), "C")
+    del C
+    W = codes(gen, 40, F)
+    C = pax_b200.gemm_i8(Q, W, s, sb[:40].contiguous(), out_dtype=F32)
+    close(C[last], gemm_i8(Q[last], W, s[last], sb[:40], None, False), "C")
+
+
 # ------------------------------------------------------------------ together
 def test_training_step_of_a_gated_layer(gen):
     """glu, the framework's own product as down-projection, and the gradients back to the input and both weights."""
