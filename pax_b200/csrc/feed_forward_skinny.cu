@@ -295,18 +295,16 @@ bool fs_shared() {
                                 (int)FsCfg<MODE, MP, R>::SMEM_BYTES) == cudaSuccess;
 }
 
-// Clusters of S CTAs that device `dev` holds at once: R times what it holds
-// with one CTA per SM, which is what the runtime answers (a cluster's CTAs
-// share a GPC, so this can be below the SMs' room).  Asked once per device,
-// kernel and S; 0: error.
-template <int MODE, int MP, int R>
+// Clusters of S CTAs that device `dev` holds at once with one CTA per SM,
+// which is what the runtime answers whatever shared memory a CTA takes (a
+// cluster's CTAs share a GPC, so this can be below the SMs' room); with R CTAs
+// per SM it is R times that.  Asked once per device and S, of one kernel for
+// all; 0: error.
 int fs_clusters(int dev, int S) {
     static int cache[64][kMaxSplit + 1] = {{0}};
     int& v = cache[dev & 63][S];
     if (v == 0) {
-        using Cfg = FsCfg<MODE, MP, R>;
-        auto kern = ff_skinny_kernel<MODE, MP, R>;
-        if (!fs_shared<MODE, MP, R>()) return 0;
+        if (!fs_shared<FS_GLU, 16, 2>()) return 0;
         cudaLaunchConfig_t cfg = {};
         cudaLaunchAttribute attr[1];
         attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -314,16 +312,16 @@ int fs_clusters(int dev, int S) {
         attr[0].val.clusterDim.y = 1;
         attr[0].val.clusterDim.z = 1;
         cfg.blockDim = dim3(192);
-        cfg.dynamicSmemBytes = Cfg::SMEM_BYTES;
+        cfg.dynamicSmemBytes = FsCfg<FS_GLU, 16, 2>::SMEM_BYTES;
         cfg.attrs = attr;
         cfg.numAttrs = 1;
         cfg.gridDim = dim3((unsigned)(4 * device_sm_count(dev) * S));  // the answer is capped by the grid
         int n = 0;
-        if (cudaOccupancyMaxActiveClusters(&n, kern, &cfg) != cudaSuccess) {
+        if (cudaOccupancyMaxActiveClusters(&n, ff_skinny_kernel<FS_GLU, 16, 2>, &cfg) != cudaSuccess) {
             cudaGetLastError();
             return 0;
         }
-        v = R * n;
+        v = n;
     }
     return v;
 }
@@ -394,7 +392,7 @@ FsPlan fs_plan(const FsParams& p) {
             // CTAs that share an SM with others take four k-blocks at least
             // (16x1024x2816 with two: 6.9 us, with four 5.7).
             if (s > 1 && (tiles * s > (long long)r * sms || p.kbs < (tiles * s > sms ? 4 : 2) * s)) break;
-            const long long n = r == 2 ? fs_clusters<MODE, MP, 2>(dev, s) : fs_clusters<MODE, MP, 3>(dev, s);
+            const long long n = (long long)r * fs_clusters(dev, s);
             if (n <= 0 || (s > 1 && tiles > n)) continue;
             const long long waves = (tiles - 1) / n;  // before the last one
             const double kb = (p.kbs + s - 1) / s;
