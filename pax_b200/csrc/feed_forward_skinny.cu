@@ -239,6 +239,19 @@ __global__ void __launch_bounds__(192, R)
         for (int m = 0; m < MP; ++m)
             if (m < M) st_shared_cluster_f32(to + (uint32_t)(m * stride * 4), v[m]);
     }
+    // A thread finishes one column of this CTA's part, for every step-th token:
+    // its scale and bias come while the contributions arrive.
+    const int pstart = part_start<TILE>(rank, S), pwidth = part_start<TILE>(rank + 1, S) - pstart;
+    int shift = 0;
+    while ((1 << shift) < pwidth) ++shift;
+    const int c = (int)threadIdx.x & ((1 << shift) - 1), step = 192 >> shift;
+    const long long col = (long long)tile * TILE + pstart + c;
+    const bool mine = (int)threadIdx.x >> shift < step && c < pwidth && col < p.N;
+    float sb = 0.f, bias = 0.f;
+    if (MODE == FS_I8 && mine) {
+        sb = __ldg(p.sb + col);
+        if (p.bias) bias = __half2float(p.bias[col]);
+    }
     __syncwarp();
     cluster_sync();  // the contributions are in; nothing remote happens after this
     if (warp == 1) {
@@ -247,17 +260,16 @@ __global__ void __launch_bounds__(192, R)
     }
     // What follows in the stream relies on the grid this one ran beside.
     if (MODE == FS_DX && p.beside && threadIdx.x == 0) pdl_wait();
-    if (*abort_flag) return;
+    if (*abort_flag || !mine) return;
     const float* r = reinterpret_cast<const float*>(smem);
-    const int pstart = part_start<TILE>(rank, S), pwidth = part_start<TILE>(rank + 1, S) - pstart;
-    for (int e = (int)threadIdx.x; e < M * pwidth; e += 192) {
-        const int m = e / pwidth, c = e - m * pwidth;
-        const long long row = m0 + m, col = (long long)tile * TILE + pstart + c;
-        if (col >= p.N) continue;
+#pragma unroll 1
+    for (int m = (int)threadIdx.x >> shift; m < M; m += step) {
+        const long long row = m0 + m;
+        const float* x = r + m * stride + c;
         if constexpr (MODE == FS_GLU) {
             float g = 0.f, u = 0.f;
-            for (int s = 0; s < S; ++s) {
-                const float* x = r + (s * M + m) * stride + c;
+#pragma unroll 1
+            for (int s = 0; s < S; ++s, x += M * stride) {
                 g += x[0];
                 u += x[pwidth];
             }
@@ -268,13 +280,16 @@ __global__ void __launch_bounds__(192, R)
             }
         } else if constexpr (MODE == FS_DX) {
             float sum = 0.f;
-            for (int s = 0; s < S; ++s) sum += r[(s * M + m) * stride + c];
+#pragma unroll 1
+            for (int s = 0; s < S; ++s, x += M * stride) sum += x[0];
             p.H[row * p.ldh + col] = __float2half_rn(sum);
         } else {
+            const float sa = __ldg(p.sa + row);
             int sum = 0;
-            for (int s = 0; s < S; ++s) sum += __float_as_int(r[(s * M + m) * stride + c]);
-            float o = (float)sum * p.sa[row] * p.sb[col];
-            if (p.bias) o += __half2float(p.bias[col]);
+#pragma unroll 1
+            for (int s = 0; s < S; ++s, x += M * stride) sum += __float_as_int(x[0]);
+            float o = (float)sum * sa * sb;
+            if (p.bias) o += bias;
             if (p.c_f16)
                 static_cast<__half*>(p.C)[row * p.ldc + col] = __float2half_rn(o);
             else
