@@ -47,6 +47,12 @@ inline bool out16(const void* p, long long cols, long long ld, int elem) {
     return rows16(p, ld, elem) && (cols * elem) % 16 == 0;
 }
 
+// The largest of 8, 4 and 2 bytes that all rows start on.
+inline int store_unit(const void* p, long long ld, int elem) {
+    const uintptr_t bits = reinterpret_cast<uintptr_t>(p) | (uintptr_t)(ld * elem);
+    return bits % 8 == 0 ? 8 : bits % 4 == 0 ? 4 : 2;
+}
+
 // feed_forward_any.cu: any layout, any alignment, empty sums.
 pax_status_t glu_any(const GluProblem& p, cudaStream_t stream);
 pax_status_t glu_dx_any(const GluGradProblem& p, cudaStream_t stream);

@@ -40,7 +40,7 @@ struct SpParams {
     long long ldc;
     const float *sa, *sb;
     const __half* bias;
-    int c_tma;
+    int c_tma, c_unit;
 };
 
 struct SpCfg {
@@ -329,17 +329,10 @@ __global__ void __launch_bounds__(SpCfg::THREADS, 1)
                     bulk_commit();
                 }
             } else {
-                // Rows of C that are not 16-byte aligned leave one after
-                // another, a warp per row.
+                // Rows of C that TMA cannot store.
                 __syncwarp();
-                const int left = min(EC, p.N - ccol), last = min(32, p.M - row0);
-                for (int i = 0; i < last; ++i) {
-                    OutT* o = static_cast<OutT*>(p.C) + (long long)(row0 + i) * p.ldc + ccol;
-                    for (int e = lane; e < left; e += 32) {
-                        const int byte = e * (int)sizeof(OutT);
-                        o[e] = *reinterpret_cast<const OutT*>(sbuf + i * 128 + (((byte >> 4) ^ (i & 7)) << 4) + (byte & 15));
-                    }
-                }
+                OutT* to = static_cast<OutT*>(p.C) + (long long)row0 * p.ldc + ccol;
+                ff_store_rows(sbuf, to, p.ldc, min(EC, p.N - ccol), min(32, p.M - row0), p.c_unit, lane);
                 __syncwarp();
             }
         }
@@ -462,6 +455,7 @@ pax_status_t gemm_i8_split(const I8Problem& q, int S, cudaStream_t stream) {
     const int ce = q.c_f16 ? 2 : 4;
     SpParams p = {};
     p.c_tma = out16(q.C, q.N, q.ldc, ce);
+    p.c_unit = store_unit(q.C, q.ldc, ce);
     if (!matrix_map(&m[0], q.A, kU8, 1, q.M, q.K, q.lda, 128, 128) || !matrix_map(&m[1], q.B, kU8, 1, q.N, q.K, q.ldb, 128, 128))
         return PAX_ERR_CUDA;
     m[2] = m[3] = m[4] = m[5] = m[0];

@@ -242,6 +242,7 @@ pax_status_t gemm_i8_tc(const I8Problem& q, cudaStream_t stream) {
               matrix_map(&m[MI_B2], q.B, kU8, 1, q.N, q.K, q.ldb, 128, 64) &&
               matrix_map(&m[MI_B4], q.B, kU8, 1, q.N, q.K, q.ldb, 128, 32);
     p.c_tma = out16(q.C, q.N, q.ldc, ce);
+    p.c_unit = store_unit(q.C, q.ldc, ce);
     m[MI_C] = m[MI_A];
     if (ok && p.c_tma) ok = matrix_map(&m[MI_C], q.C, q.c_f16 ? kF16 : kF32, ce, q.M, q.N, q.ldc, 128 / ce, 32);
     if (!ok) return PAX_ERR_CUDA;

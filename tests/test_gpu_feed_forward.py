@@ -340,6 +340,20 @@ def test_gemm_i8_strided(gen, M, out):
     close(C, gemm_i8(A, B, sa, sb, None, out == F16), "C")
 
 
+@pytest.mark.parametrize("M,K", [(200, 144), (300, 2064)])
+@pytest.mark.parametrize("N", [129, 130, 131, 201, 318])
+@pytest.mark.parametrize("out", [F16, F32])
+def test_gemm_i8_rows_on_2_4_and_8_bytes(gen, M, K, N, out):
+    """Every alignment of the output's rows, their last element anywhere in a unit; what follows the rows stays."""
+    A, B = codes(gen, M, K), codes(gen, N, K)
+    sa, sb = torch.rand(M, generator=gen, device=gen.device) * 1e-2, torch.rand(N, generator=gen, device=gen.device) * 1e-2
+    ref = gemm_i8(A, B, sa, sb, None, out == F16)
+    for wide in (N + 1, N + 2, N + 3, N + 4):
+        buf = torch.full((M + 1, wide), 7.0, device=gen.device, dtype=out)
+        close(pax_b200.gemm_i8(A, B, sa, sb, out=buf[:M, :N]), ref, "C")
+        assert (buf[:, N:] == 7).all() and (buf[M] == 7).all()
+
+
 @pytest.mark.parametrize("M", [3, 80])
 def test_gemm_i8_empty_sum_and_scales_that_are_not_finite(gen, M):
     one = lambda n: torch.ones(n, device=gen.device)  # noqa: E731
