@@ -295,14 +295,15 @@ __global__ void __launch_bounds__(64 + 32 * 8, 1)
     tc_fence_after();
     const uint32_t tmem_base = *tmem_slot;
     const int num_kb = (p.K + Cfg::BK - 1) / Cfg::BK;
-    // A following kernel launched with programmatic serialization may start
-    // its prologue now; it waits for this grid before touching memory.
-    if (threadIdx.x == 0) pdl_launch_dependents();
 
     if (warp == 0) {
         // ------------------------------------------------ TMA producer
         if (lane == 0) {
             pdl_wait();  // A and B may be written by the previous grid
+            // A following kernel launched with programmatic serialization may
+            // start now; not before, since it may load a constant B early,
+            // which the grid before this one may still be writing.
+            pdl_launch_dependents();
             int stage = 0;
             uint32_t phase = 0;
             bool ok = true;
