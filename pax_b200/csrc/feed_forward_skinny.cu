@@ -121,7 +121,6 @@ __global__ void __launch_bounds__(192, R)
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem_base = *tmem_slot;
-    if (threadIdx.x == 0) pdl_launch_dependents();
 
     float v[MP];
     const int q = warp & 3;  // TMEM lane quarter an epilogue warp may read
@@ -159,7 +158,12 @@ __global__ void __launch_bounds__(192, R)
                     load_weights(kb);
                 }
             stage = 0;
-            if (MODE != FS_DX || !p.beside) pdl_wait();  // the operands may be written by the previous grid
+            if (MODE != FS_DX || !p.beside) {
+                pdl_wait();  // the operands may be written by the previous grid
+                // Not before: the next grid may load weights early, which only
+                // this grid is known not to write.
+                pdl_launch_dependents();
+            }
             for (int kb = rank; kb < p.kbs; kb += S) {
                 if (!mbar_wait(empty0 + 8u * stage, phase ^ 1u, abort_flag)) break;
                 const bool have = total < early;
@@ -259,7 +263,10 @@ __global__ void __launch_bounds__(192, R)
         tmem_dealloc<1>(tmem_base, Cfg::TMEM_COLS);
     }
     // What follows in the stream relies on the grid this one ran beside.
-    if (MODE == FS_DX && p.beside && threadIdx.x == 0) pdl_wait();
+    if (MODE == FS_DX && p.beside && threadIdx.x == 0) {
+        pdl_wait();
+        pdl_launch_dependents();
+    }
     if (*abort_flag || !mine) return;
     const float* r = reinterpret_cast<const float*>(smem);
 #pragma unroll 1

@@ -109,15 +109,12 @@ __global__ void __launch_bounds__(SpCfg::THREADS, 1)
     cluster_sync();
     tc_fence_after();
     const uint32_t tmem_base = *tmem_slot;
-    if (MODE != SP_DW && threadIdx.x == 0) pdl_launch_dependents();
 
     if (warp == 0) {
         // ------------------------------------------------ TMA producer
         if (lane == 0) {
             pdl_wait();  // the operands may be written by the previous grid
-            // SP_DW: as FF_BACK's, a kernel that starts early finds dG and dU
-            // written.
-            if (MODE == SP_DW) pdl_launch_dependents();
+            pdl_launch_dependents();  // not before, as in ff_tc_kernel
             int stage = 0, total = 0;
             uint32_t phase = 0;
             for (int kb = pair; kb < p.kbs; kb += S) {

@@ -278,15 +278,15 @@ __global__ void __launch_bounds__(FfCfg<MODE, W>::THREADS, 1)
     cluster_sync();  // barrier initialisation visible to the peer CTA
     tc_fence_after();
     const uint32_t tmem_base = *tmem_slot;
-    if (MODE != FF_BACK && threadIdx.x == 0) pdl_launch_dependents();
 
     if (warp == 0) {
         // ------------------------------------------------ TMA producer
         if (lane == 0) {
             pdl_wait();  // the operands may be written by the previous grid
-            // FF_BACK: a kernel that starts early finds dG and dU written,
-            // since the grid that wrote them has ended (glu_dx_skinny).
-            if (MODE == FF_BACK) pdl_launch_dependents();
+            // Not before: what the next grid loads early (weights) is known not
+            // to be written by this grid, but may be by the one before it, and
+            // glu_dx_skinny relies on dG and dU being written.
+            pdl_launch_dependents();
             int stage = 0, total = 0;
             uint32_t phase = 0;
             bool ok = true;

@@ -522,6 +522,27 @@ def test_backward_passes_in_a_row_with_inputs_that_change(gen, shape):
     assert wrong.item() == 0
 
 
+@pytest.mark.parametrize("between", ["glu, few tokens", "glu, tiles", "glu, split", "gemm_i8, tiles", "gemm, tiles", "gemm, few rows"])
+def test_constant_weights_written_by_the_kernel_before_the_one_just_before(gen, between):
+    """Three kernels in a row: the first writes B, the second is small and leaves most of the GPU free, the third has b_const."""
+    N = K = 8192
+    W, A = randn(gen, N, K), codes(gen, 1, K)
+    ones = torch.ones(N, device=gen.device)
+    Q, s = pax_b200.quantize_rows(W)
+    ref = pax_b200.gemm_i8(A, Q, ones[:1], ones, out_dtype=F32)
+    M, D, F = {"glu, few tokens": (1, 64, 64), "glu, split": (256, 2048, 128)}.get(between, (256, 64, 128))
+    X, Y = randn(gen, M, D), randn(gen, D, F)
+    A2, B2, s2, C = codes(gen, M, D), codes(gen, F, D), ones[:M], torch.empty((M, F), device=gen.device, dtype=F32)
+    second = {"glu": lambda: pax_b200.glu(X, Y, Y), "gemm_i8": lambda: pax_b200.gemm_i8(A2, B2, s2, ones[:F]),
+              "gemm": lambda: pax_b200.gemm(X if "tiles" in between else X[:4], Y, out=C if "tiles" in between else C[:4])}
+    second = second[between.split(",")[0]]
+    for _ in range(10):
+        Q.fill_(1)
+        pax_b200.quantize_rows(W, out=Q, scale=s)
+        second()
+        assert torch.equal(pax_b200.gemm_i8(A, Q, ones[:1], ones, out_dtype=F32, b_const=True), ref)
+
+
 @pytest.mark.parametrize("M", [1, 24, 64])
 def test_decoding_chain_with_constant_weights(gen, M):
     """Layers in a row, each reading what the one before wrote, with their weights marked constant: the same bits as without."""
