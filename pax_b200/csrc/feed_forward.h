@@ -47,6 +47,12 @@ inline bool out16(const void* p, long long cols, long long ld, int elem) {
     return rows16(p, ld, elem) && (cols * elem) % 16 == 0;
 }
 
+// The longest sum the kernels with bounded waits take: a tile's k-blocks, 2^20
+// of 64 (two terms: 2^21), end in about 0.8 s (1.3 s in wide tiles), below the
+// waits' limit of 2 s.  Longer ones run on the any-layout kernel, which waits
+// for nothing.
+constexpr long long kMaxSum = 1LL << 26;
+
 // The largest of 8, 4 and 2 bytes that all rows start on.
 inline int store_unit(const void* p, long long ld, int elem) {
     const uintptr_t bits = reinterpret_cast<uintptr_t>(p) | (uintptr_t)(ld * elem);

@@ -31,6 +31,8 @@
 #include "feed_forward.h"
 #include "tmap.h"
 
+#include <atomic>
+
 namespace pax {
 
 namespace {
@@ -308,7 +310,6 @@ __global__ void __launch_bounds__(192, R)
 // ------------------------------------------------------------------ host
 constexpr int kMaxSplit = 8;
 
-
 // Allow the kernel its shared memory on the current device: per device and
 // context, and cheap to repeat.
 template <int MODE, int MP, int R>
@@ -323,8 +324,8 @@ bool fs_shared() {
 // per SM it is R times that.  Asked once per device and S, of one kernel for
 // all; 0: error.
 int fs_clusters(int dev, int S) {
-    static int cache[64][kMaxSplit + 1] = {{0}};
-    int& v = cache[dev & 63][S];
+    static std::atomic<int> cache[64][kMaxSplit + 1];  // zero; calls may come from several threads
+    std::atomic<int>& v = cache[dev & 63][S];
     if (v == 0) {
         if (!fs_shared<FS_GLU, 16, 2>()) return 0;
         cudaLaunchConfig_t cfg = {};
@@ -468,7 +469,7 @@ int chunk_rows(long long M) {
 constexpr long long kMaxChunked = 512;
 
 bool glu_skinny_ok(const GluProblem& q) {
-    return q.M <= kMaxChunked && q.D > 0 && rows16(q.X, q.ldx, 2) && rows16(q.Wg, q.ldwg, 2) && rows16(q.Wu, q.ldwu, 2);
+    return q.M <= kMaxChunked && q.D > 0 && q.D <= kMaxSum && rows16(q.X, q.ldx, 2) && rows16(q.Wg, q.ldwg, 2) && rows16(q.Wu, q.ldwu, 2);
 }
 
 static void glu_params(const GluProblem& q, FsParams& p) {
@@ -500,7 +501,7 @@ pax_status_t glu_skinny(const GluProblem& q, cudaStream_t stream) {
 }
 
 bool glu_dx_skinny_ok(const GluGradProblem& q) {
-    return q.dX && q.M > 0 && q.M <= 64LL * 65535 && q.D > 0 && q.F > 0 && rows16(q.dG, q.lddg, 2) &&
+    return q.dX && q.M > 0 && q.M <= 64LL * 65535 && q.D > 0 && q.F > 0 && q.F <= kMaxSum && rows16(q.dG, q.lddg, 2) &&
            rows16(q.dU, q.lddu, 2) && rows16(q.Wg, q.ldwg, 2) && rows16(q.Wu, q.ldwu, 2);
 }
 

@@ -347,8 +347,8 @@ bool sp_shared() {
 // Clusters of 2 S CTAs that a device holds at once, asked once per device.
 // The kernels are alike in what that depends on (one CTA per SM).
 int sp_clusters(int dev, int S) {
-    static int cache[64][5] = {{0}};
-    int& v = cache[dev & 63][S];
+    static std::atomic<int> cache[64][5];  // zero
+    std::atomic<int>& v = cache[dev & 63][S];
     if (v == 0) {
         if (!sp_shared<SP_DX, 0, __half>()) return 0;
         cudaLaunchConfig_t cfg = {};

@@ -121,7 +121,7 @@ bool tiles_ok(long long a, long long b) { return a * b <= 0x3fffffffLL; }
 }  // namespace
 
 bool glu_tc_ok(const GluProblem& q) {
-    return q.D > 0 && rows16(q.X, q.ldx, 2) && rows16(q.Wg, q.ldwg, 2) && rows16(q.Wu, q.ldwu, 2) &&
+    return q.D > 0 && q.D <= kMaxSum && rows16(q.X, q.ldx, 2) && rows16(q.Wg, q.ldwg, 2) && rows16(q.Wu, q.ldwu, 2) &&
            out16(q.H, q.F, q.ldh, 2) && (!q.G || (out16(q.G, q.F, q.ldg, 2) && out16(q.U, q.F, q.ldu, 2))) &&
            tiles_ok(up(q.M, 256), up(q.F, 128));
 }
@@ -166,8 +166,8 @@ pax_status_t glu_tc(const GluProblem& q, cudaStream_t stream) {
 bool glu_back_tc_ok(const GluGradProblem& q) {
     const int w = q.dw_f16 ? 2 : 4;
     return q.M > 0 && q.D > 0 && q.F > 0 && rows16(q.dG, q.lddg, 2) && rows16(q.dU, q.lddu, 2) &&
-           (!q.dX || (rows16(q.Wg, q.ldwg, 2) && rows16(q.Wu, q.ldwu, 2) && out16(q.dX, q.D, q.lddx, 2))) &&
-           (!q.dWg || (rows16(q.X, q.ldx, 2) && out16(q.dWg, q.F, q.lddwg, w) && out16(q.dWu, q.F, q.lddwu, w))) &&
+           (!q.dX || (q.F <= kMaxSum && rows16(q.Wg, q.ldwg, 2) && rows16(q.Wu, q.ldwu, 2) && out16(q.dX, q.D, q.lddx, 2))) &&
+           (!q.dWg || (q.M <= kMaxSum && rows16(q.X, q.ldx, 2) && out16(q.dWg, q.F, q.lddwg, w) && out16(q.dWu, q.F, q.lddwu, w))) &&
            tiles_ok(up(q.M, 256), up(q.D, 256)) && tiles_ok(up(q.D, 256), 2LL * up(q.F, 256));
 }
 

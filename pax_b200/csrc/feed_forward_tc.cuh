@@ -35,6 +35,7 @@
 #include "feed_forward.h"
 #include "tmap.h"
 
+#include <atomic>
 #include <type_traits>
 
 namespace pax {
@@ -652,8 +653,8 @@ inline bool ff_shared() {
 // kernel.
 template <int MODE, int ACT, typename OutT, int W>
 inline int ff_units(int dev) {
-    static int cache[64] = {0};
-    int& v = cache[dev & 63];
+    static std::atomic<int> cache[64];  // zero; calls may come from several threads
+    std::atomic<int>& v = cache[dev & 63];
     if (v == 0) {
         auto kern = ff_tc_kernel<MODE, ACT, OutT, W>;
         if (!ff_shared<MODE, ACT, OutT, W>()) return 0;

@@ -7,6 +7,7 @@ pax_gemm_i8_ex).
 Every call is asynchronous on the current stream of the tensors' device, or on
 ``stream``, whatever device is current.  A new output belongs to that stream:
 a caller that passes ``stream`` orders its own use of the output after it.
+Outputs must not overlap inputs or each other, but for glu_backward's dG and dU.
 autograd records none of the calls: glu_backward is called by hand.
 """
 from __future__ import annotations

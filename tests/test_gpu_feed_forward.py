@@ -522,6 +522,20 @@ def test_backward_passes_in_a_row_with_inputs_that_change(gen, shape):
     assert wrong.item() == 0
 
 
+def test_glu_backward_sums_over_more_tokens_than_a_bounded_wait_covers(gen):
+    """One term in 2^20 tokens is not zero and every product of them is exact, so that the sums are too."""
+    M = (1 << 26) + 72
+    X, G, U, dH = (torch.zeros(M, 8, device=gen.device, dtype=F16) for _ in range(4))
+    X[:: 1 << 20] = 2.0
+    U[:: 1 << 20] = 1.0
+    dH[:: 1 << 20] = 1.0
+    W = torch.zeros(8, 8, device=gen.device, dtype=F16)
+    _, dWg, dWu = pax_b200.glu_backward(dH, X, W, W.clone(), G, U, need_dX=False, dW_dtype=F32, dG=G, dU=U)
+    # silu'(0) = 1/2 and silu(0) = 0: 65 tokens of 2 * 1/2
+    assert (dWg == 65.0).all() and (dWu == 0).all()
+    assert pax_b200.device_error() == pax_b200.Status.OK
+
+
 @pytest.mark.parametrize("between", ["glu, few tokens", "glu, tiles", "glu, split", "gemm_i8, tiles", "gemm, tiles", "gemm, few rows"])
 def test_constant_weights_written_by_the_kernel_before_the_one_just_before(gen, between):
     """Three kernels in a row: the first writes B, the second is small and leaves most of the GPU free, the third has b_const."""
