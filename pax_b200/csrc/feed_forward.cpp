@@ -74,8 +74,12 @@ pax_status_t back_products(const GluGradProblem& p, cudaStream_t stream) {
     x.dWg = x.dWu = nullptr;
     w.dX = nullptr;
     const SplitPlan xs = glu_dx_split_plan(p), ws = glu_dw_split_plan(p);
-    const double few = 1.3 * glu_dx_skinny_time(p) + 8.0, wt = glu_back_tc_time(w);
-    const double x_time = few < xs.time ? few : xs.time, w_time = wt < ws.time ? wt : ws.time;
+    // A kernel that cannot run dX's shape has no time: dX apart is then left to
+    // the tiles (8388608x64x64: too many chunks, too few k-blocks to split).
+    const bool chunked = p.M <= kMaxChunkedTokens, split = xs.S > 0;
+    const double few = chunked ? 1.3 * glu_dx_skinny_time(p) + 8.0 : 1e30, wt = glu_back_tc_time(w);
+    const double x_time = !chunked && !split ? glu_back_tc_time(x) : few < xs.time ? few : xs.time;
+    const double w_time = wt < ws.time ? wt : ws.time;
     const bool apart = x_time + w_time + 6.0 < glu_back_tc_time(both);
 
     GluGradProblem px = p, pw = p;  // each part as asked for
@@ -97,7 +101,7 @@ pax_status_t back_products(const GluGradProblem& p, cudaStream_t stream) {
     const bool tiles_ok = glu_back_tc_ok(px);
     if (glu_dx_skinny_ok(p) && (!tiles_ok || (apart && few < xs.time))) return glu_dx_skinny(p, beside, stream);
     if (!tiles_ok) return glu_dx_any(px, stream);
-    return apart ? glu_dx_split(px, xs.S, stream) : glu_back_tc(px, stream);
+    return apart && split ? glu_dx_split(px, xs.S, stream) : glu_back_tc(px, stream);
 }
 
 pax_status_t done(pax_status_t st, const char* who) {

@@ -53,6 +53,10 @@ inline bool out16(const void* p, long long cols, long long ld, int elem) {
 // for nothing.
 constexpr long long kMaxSum = 1LL << 26;
 
+// The most tokens that the few-token kernel's chunks of 64 cover: a grid has
+// 65535 of them.
+constexpr long long kMaxChunkedTokens = 64LL * 65535;
+
 // The largest of 8, 4 and 2 bytes that all rows start on.
 inline int store_unit(const void* p, long long ld, int elem) {
     const uintptr_t bits = reinterpret_cast<uintptr_t>(p) | (uintptr_t)(ld * elem);

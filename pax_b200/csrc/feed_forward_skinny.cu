@@ -501,7 +501,7 @@ pax_status_t glu_skinny(const GluProblem& q, cudaStream_t stream) {
 }
 
 bool glu_dx_skinny_ok(const GluGradProblem& q) {
-    return q.dX && q.M > 0 && q.M <= 64LL * 65535 && q.D > 0 && q.F > 0 && q.F <= kMaxSum && rows16(q.dG, q.lddg, 2) &&
+    return q.dX && q.M > 0 && q.M <= kMaxChunkedTokens && q.D > 0 && q.F > 0 && q.F <= kMaxSum && rows16(q.dG, q.lddg, 2) &&
            rows16(q.dU, q.lddu, 2) && rows16(q.Wg, q.ldwg, 2) && rows16(q.Wu, q.ldwu, 2);
 }
 
