@@ -60,7 +60,9 @@ __device__ __forceinline__ float rcp_approx(float x) {
     asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
-__device__ __forceinline__ float erfc_hastings(float w) {  // 1 - erf(w), w >= 0
+__device__ __forceinline__ float gelu_erf(float x) {
+    const float z = x * 0.70710678118654752f;
+    const float w = fabsf(z);
     float p = fmaf(w, 4.30638e-5f, 2.765672e-4f);
     p = fmaf(p, w, 1.520143e-4f);
     p = fmaf(p, w, 9.2705272e-3f);
@@ -70,12 +72,8 @@ __device__ __forceinline__ float erfc_hastings(float w) {  // 1 - erf(w), w >= 0
     p *= p;
     p *= p;
     p *= p;
-    p *= p;                // p^16 (inf for |z| above about 19: q = 0)
-    return rcp_approx(p);
-}
-__device__ __forceinline__ float gelu_erf(float x) {
-    const float z = x * 0.70710678118654752f;
-    const float q = erfc_hastings(fabsf(z));
+    p *= p;                         // p^16 (inf for |z| above about 19: q = 0)
+    const float q = rcp_approx(p);  // 1 - erf(w)
     return 0.5f * x * (z >= 0.f ? 2.0f - q : q);
 }
 

@@ -33,11 +33,10 @@ __device__ __forceinline__ void grad8(const uint4& vh, const uint4& vg, const ui
     uint32_t g[4], u[4];
 #pragma unroll
     for (int i = 0; i < 8; i += 2) {
-        float v0, d0, v1, d1;
-        act_value_grad<ACT>(a[i], v0, d0);
-        act_value_grad<ACT>(a[i + 1], v1, d1);
-        g[i / 2] = pack_half2(h[i] * b[i] * d0, h[i + 1] * b[i + 1] * d1);
-        u[i / 2] = pack_half2(h[i] * v0, h[i + 1] * v1);
+        float2 v, d;
+        act_value_grad2<ACT>(make_float2(a[i], a[i + 1]), v, d);
+        g[i / 2] = pack_half2(h[i] * b[i] * d.x, h[i + 1] * b[i + 1] * d.y);
+        u[i / 2] = pack_half2(h[i] * v.x, h[i + 1] * v.y);
     }
     og = make_uint4(g[0], g[1], g[2], g[3]);
     ou = make_uint4(u[0], u[1], u[2], u[3]);
@@ -85,10 +84,10 @@ __global__ void __launch_bounds__(kGradThreads) glu_grad_kernel(const GluGradPro
                 const long long r = row, c = j - row * per_row;
                 const float h = __half2float(p.dH[r * p.lddh + c]), a = __half2float(p.G[r * p.ldg + c]);
                 const float b = __half2float(p.U[r * p.ldu + c]);
-                float v, d;
-                act_value_grad<ACT>(a, v, d);
-                p.dG[r * p.lddg + c] = __float2half_rn(h * b * d);
-                p.dU[r * p.lddu + c] = __float2half_rn(h * v);
+                float2 v, d;
+                act_value_grad2<ACT>(make_float2(a, a), v, d);
+                p.dG[r * p.lddg + c] = __float2half_rn(h * b * d.x);
+                p.dU[r * p.lddu + c] = __float2half_rn(h * v.x);
             }
         }
     }

@@ -290,7 +290,11 @@ __global__ void __launch_bounds__(SpCfg::THREADS, 1)
                         float u[8];
                         sum8(128 + c0 + c, u);
 #pragma unroll
-                        for (int i = 0; i < 8; ++i) v[i] = act_value<ACT>(v[i]) * u[i];
+                        for (int i = 0; i < 8; i += 2) {
+                            const float2 a = act_value2<ACT>(make_float2(v[i], v[i + 1]));
+                            v[i] = a.x * u[i];
+                            v[i + 1] = a.y * u[i + 1];
+                        }
                     }
                 } else {
                     sum8(c0 + c, v);

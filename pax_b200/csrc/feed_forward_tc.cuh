@@ -534,8 +534,8 @@ __global__ void __launch_bounds__(FfCfg<MODE, W>::THREADS, 1)
                         for (int i = 0; i < 16; ++i) {
                             wG[16 * h + i] = pack_half2(g[2 * i], g[2 * i + 1]);
                             wU[16 * h + i] = pack_half2(u[2 * i], u[2 * i + 1]);
-                            wH[16 * h + i] = pack_half2(act_value<ACT>(g[2 * i]) * u[2 * i],
-                                                        act_value<ACT>(g[2 * i + 1]) * u[2 * i + 1]);
+                            const float2 a = act_value2<ACT>(make_float2(g[2 * i], g[2 * i + 1]));
+                            wH[16 * h + i] = pack_half2(a.x * u[2 * i], a.y * u[2 * i + 1]);
                         }
                     }
                     store(&maps.m[MG_H], wH, col, row0, false);

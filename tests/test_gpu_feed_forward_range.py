@@ -7,6 +7,7 @@ import pytest
 import torch
 
 import pax_b200
+from _feed_forward import ACTS
 
 pytestmark = pytest.mark.gpu
 F16, F32, I8 = torch.float16, torch.float32, torch.int8
@@ -44,3 +45,70 @@ def test_glu_backward_of_more_tokens_than_chunks_of_a_grid(gen, shape, parts):
         want = sum(x.double().T @ h.double() for x, h in zip(X.split(1 << 20), (dH / 2).split(1 << 20)))
         assert torch.equal(dWg.double(), want + 1)
     assert pax_b200.device_error() == pax_b200.Status.OK
+
+
+# ------------------------------------------------------------------ the gate's whole range
+def gate_parts(x, name):
+    """64-bit act(x), act'(x), the sum of the magnitudes of act's two terms, and the bound on the relative error of each term.
+
+    sigmoid(y) = 1 / (1 + exp(-y)): y takes up to 5 roundings of 2^-24, the exponential's base-2 argument 1 more, which the
+    exponential turns into up to 6 |y| of them; the exponential, the sum, the reciprocal and the products are good to 2 or 3
+    each, below 16 in all.  erfc: 3 roundings of its argument x^2 / 2, below 24 for polynomial and products.  Below
+    y = -104 the true value is under 2^-149."""
+    if name == "gelu_erf":
+        cdf, phi = 0.5 * torch.special.erfc(-x / 2 ** 0.5), torch.exp(-0.5 * x * x) / (2 * torch.pi) ** 0.5
+        a, d1, d2, y = x * cdf, cdf, x * phi, 0.5 * x * x
+    else:
+        k = 2 * (2 / torch.pi) ** 0.5
+        y = x if name == "silu" else k * (x + 0.044715 * x ** 3)
+        dy = 1.0 if name == "silu" else k * (1 + 3 * 0.044715 * x * x)
+        p, q = torch.sigmoid(y), torch.sigmoid(-y)
+        a, d1, d2 = x * p, p, x * p * q * dy
+    return a, d1 + d2, d1.abs() + d2.abs(), 2.0 ** -24 * (32 + 8 * y.abs().clamp_max(104.0))
+
+
+def whole_range(gen, n):
+    """n fp16 values of both signs: every magnitude from 2^-24 to 65504, and half of them in the steep part and the tails."""
+    wide = torch.logspace(-7.2, 4.816, n // 4, device=gen.device, dtype=torch.float64).clamp_max(65504.0)
+    near = torch.linspace(0, 14, n // 2 - n // 4, device=gen.device, dtype=torch.float64)
+    m = torch.cat([wide, near]).half()
+    return torch.cat([m, -m])[torch.randperm(n, generator=gen, device=gen.device)]
+
+
+@pytest.mark.parametrize("name", ACTS)
+@pytest.mark.parametrize("up", [1.0, 1000.0])
+@pytest.mark.parametrize("M,pad", [(5, 0), (200, 0), (1200, 0), (60, 1)])
+def test_glu_keeps_the_gates_tails(gen, name, up, M, pad):
+    """One term a sum, so that G and U are exact and H is off by the gate's own relative error and one rounding."""
+    D, F = 64, 1024 + pad
+    X = torch.eye(D, device=gen.device, dtype=F16).repeat(M // D + 1, 1)[:M].contiguous()
+    Wg, Wu = whole_range(gen, D * 1024).view(D, 1024)[:, torch.arange(F, device=gen.device) % 1024].contiguous(), randn(gen, D, F, scale=up)
+    H, G, U = pax_b200.glu(X, Wg, Wu, activation=name, save=True)
+    g, u = (X.double() @ w.double() for w in (Wg, Wu))
+    assert torch.equal(G.double(), g) and torch.equal(U.double(), u)
+    a, _, _, rel = gate_parts(g, name)
+    h = a * u
+    fits = h.abs() < 65000  # beyond fp16 a right result is an infinity
+    t = (rel + 2.0 ** -24) * h.abs()
+    tol = t + 2.0 ** -11 * (h.abs() + t) + 2.0 ** -25
+    bad = ((H.double() - h).abs() > tol) & fits
+    assert not bad.any(), (int(bad.sum()), g[bad][0].item(), H[bad][0].item(), h[bad][0].item())
+
+
+@pytest.mark.parametrize("name", ACTS)
+@pytest.mark.parametrize("size", [1.0, 1000.0])
+@pytest.mark.parametrize("shape", [(64, 1024), (63, 1025)])
+def test_glu_backward_keeps_the_gates_tails(gen, name, size, shape):
+    """dG and dU over every magnitude of G: each off by its terms' relative error and one rounding."""
+    M, F = shape
+    G, U, dH = whole_range(gen, 65536).repeat(2)[: M * F].view(M, F).contiguous(), randn(gen, M, F), randn(gen, M, F, scale=size)
+    X, W = torch.zeros(M, 8, device=gen.device, dtype=F16), torch.zeros(8, F, device=gen.device, dtype=F16)
+    dG, dU = torch.empty_like(G), torch.empty_like(G)
+    pax_b200.glu_backward(dH, X, W, W.clone(), G, U, activation=name, need_dX=False, need_dW=False, dG=dG, dU=dU)
+    g, u, dh = G.double(), U.double(), dH.double()
+    a, d, terms, rel = gate_parts(g, name)
+    for what, got, want, t in (("dG", dG, dh * u * d, (dh * u).abs() * terms), ("dU", dU, dh * a, (dh * a).abs())):
+        t = (rel + 2.0 ** -23) * t
+        tol = t + 2.0 ** -11 * (want.abs() + t) + 2.0 ** -25
+        bad = ((got.double() - want).abs() > tol) & (want.abs() < 65000)
+        assert not bad.any(), (what, int(bad.sum()), g[bad][0].item(), got[bad][0].item(), want[bad][0].item())
