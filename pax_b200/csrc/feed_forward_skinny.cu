@@ -468,6 +468,11 @@ int chunk_rows(long long M) {
 // More tokens than this never read the weights again for another chunk.
 constexpr long long kMaxChunked = 512;
 
+// Constant weights are loaded early for one chunk at most, as w_const says:
+// what a caller orders by the number of tokens does not depend on which kernel
+// more of them run on.
+constexpr long long kMaxEarly = 64;
+
 bool glu_skinny_ok(const GluProblem& q) {
     return q.M <= kMaxChunked && q.D > 0 && q.D <= kMaxSum && rows16(q.X, q.ldx, 2) && rows16(q.Wg, q.ldwg, 2) && rows16(q.Wu, q.ldwu, 2);
 }
@@ -493,7 +498,7 @@ pax_status_t glu_skinny(const GluProblem& q, cudaStream_t stream) {
         !matrix_map(&m.x0, q.X, kF16, 2, q.M, q.D, q.ldx, 64, (uint32_t)p.rows))
         return PAX_ERR_CUDA;
     m.x1 = m.x0;
-    p.w_const = q.w_const;
+    p.w_const = q.w_const && q.M <= kMaxEarly;
     p.H = q.H, p.G = q.G, p.U = q.U;
     p.ldh = q.ldh, p.ldg = q.ldg, p.ldu = q.ldu;
     p.act = q.act;
@@ -563,7 +568,7 @@ pax_status_t gemm_i8_skinny(const I8Problem& q, cudaStream_t stream) {
         return PAX_ERR_CUDA;
     m.w1 = m.w0;
     m.x1 = m.x0;
-    p.w_const = q.b_const;
+    p.w_const = q.b_const && q.M <= kMaxEarly;
     p.C = q.C;
     p.ldc = q.ldc;
     p.sa = q.a_scale, p.sb = q.b_scale, p.bias = q.bias;
