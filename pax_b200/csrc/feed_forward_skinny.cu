@@ -187,6 +187,9 @@ __global__ void __launch_bounds__(192, R)
     } else if (warp == 1) {
         // ------------------------------------------------ MMA issuer
         if (lane == 0) {
+            // The waits below count from here: for the loads of this grid, not
+            // for the end of the previous one.
+            if (MODE != FS_DX || !p.beside) pdl_wait();
             int stage = 0;
             uint32_t phase = 0;
             // Weights: MN-major, two blocks of 64 columns x 64 rows, or

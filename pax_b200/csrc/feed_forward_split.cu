@@ -171,6 +171,7 @@ __global__ void __launch_bounds__(SpCfg::THREADS, 1)
     } else if (warp == 1) {
         // ------------------------------------------------ MMA issuer
         if (lane == 0 && leader) {
+            pdl_wait();  // the waits below count from the previous grid's end
             constexpr bool a_n = MODE == SP_DW, b_n = MODE == SP_GLU || MODE == SP_DW;
             const uint64_t a0 = umma_desc_sw128(smem_u32(sA), a_n ? 8192 : 16, 1024);
             const uint64_t b0 = umma_desc_sw128(smem_u32(sB), b_n ? 8192 : 16, 1024);

@@ -385,6 +385,9 @@ __global__ void __launch_bounds__(FfCfg<MODE, W>::THREADS, 1)
     } else if (warp == 1) {
         // ------------------------------------------------ MMA issuer
         if (lane == 0 && leader) {
+            // The waits below count from here: for the loads of this grid, not
+            // for the end of the previous one.
+            pdl_wait();
             int stage = 0, acc = 0;
             uint32_t phase = 0, acc_phase = 0;
             bool ok = true;

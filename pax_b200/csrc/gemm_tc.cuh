@@ -439,6 +439,9 @@ __global__ void __launch_bounds__(64 + 32 * 8, 1)
     } else if (warp == 1) {
         // ------------------------------------------------ MMA issuer (leader only in pair mode)
         if (lane == 0 && leader) {
+            // The waits below count from here: for the loads of this grid, not
+            // for the end of the previous one.
+            pdl_wait();
             int stage = 0;
             uint32_t phase = 0;
             int acc = 0;

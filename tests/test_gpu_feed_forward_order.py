@@ -52,3 +52,44 @@ def test_chain_in_chunks_with_constant_weights(gen, M):
     want = chain(False)
     for _ in range(20):
         assert torch.equal(chain(True), want)
+
+
+LONG = {"quantize_rows, one long row": 0, "quantize_rows, one long odd row": 1, "glu_backward, few tiles of many tokens": 2}
+
+
+@pytest.mark.parametrize("before", LONG)
+@pytest.mark.parametrize("after", ["glu, few tokens", "glu, tiles", "glu, split", "glu_backward", "gemm_i8, tiles", "gemm, tiles", "gemm, few rows"])
+def test_waits_count_from_the_end_of_the_kernel_before(cuda, before, after):
+    """A kernel of several milliseconds that leaves most of the GPU free, so that the next one is resident long before its
+    inputs are ready: with a limit of half a millisecond none of its waits may run out."""
+    g = torch.Generator(device=cuda)
+    g.manual_seed(5)
+    kind = LONG[before]
+    if kind < 2:
+        row = randn(g, 1, (1 << 26) + 8 - kind)
+        first = lambda: pax_b200.quantize_rows(row)  # noqa: E731
+    else:
+        tall = [randn(g, 1 << 21, 8) for _ in range(4)]
+        small = [randn(g, 8, 8) for _ in range(2)]
+        first = lambda: pax_b200.glu_backward(tall[0], tall[1], *small, *tall[2:], need_dX=False)  # noqa: E731
+    M, D, F = {"glu, few tokens": (16, 1024, 512), "glu, tiles": (512, 128, 512), "glu, split": (256, 2048, 128)}.get(after, (512, 128, 512))
+    X, Wg, Wu, G, U, dH = randn(g, M, D), randn(g, D, F), randn(g, D, F), randn(g, M, F), randn(g, M, F), randn(g, M, F)
+    A, B, sa, sb = codes(g, M, D), codes(g, F, D), torch.ones(M, device=cuda), torch.ones(F, device=cuda)
+    second = {"glu": lambda: pax_b200.glu(X, Wg, Wu), "glu_backward": lambda: pax_b200.glu_backward(dH, X, Wg, Wu, G, U)[0],
+              "gemm_i8": lambda: pax_b200.gemm_i8(A, B, sa, sb),
+              "gemm": lambda: pax_b200.gemm(X if "tiles" in after else X[:4], Wg)}[after.split(",")[0]]
+    first()
+    want = second()
+    torch.cuda.synchronize()
+    lib = pax_b200.lib
+    assert pax_b200.device_error() == pax_b200.Status.OK
+    assert lib.pax_selftest_set_wait_limit(500_000) == 0
+    try:
+        for _ in range(2):
+            first()
+            got = second()
+            torch.cuda.synchronize()
+            assert pax_b200.device_error() == pax_b200.Status.OK
+            assert torch.equal(got, want)
+    finally:
+        assert lib.pax_selftest_set_wait_limit(0) == 0
