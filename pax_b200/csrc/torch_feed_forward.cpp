@@ -114,7 +114,8 @@ int64_t attribute(PyObject* o, const char* name) {
 // The device and stream of one call.  Outputs are allocated on the call's
 // stream, so that neither their memory's earlier use nor its reuse after them
 // can overlap the call, and stay reserved for the caller's current stream as
-// well.
+// well.  What the caller gives stays reserved for the call's stream until it is
+// done there, also where the caller frees it right after the call.
 class Call {
 public:
     Call(c10::Device dev, PyObject* stream)
@@ -130,6 +131,12 @@ public:
         at::Tensor t = at::detail::empty_cuda(shape, dtype, dev_, std::nullopt);
         if (!scratch && t.numel()) c10::cuda::CUDACachingAllocator::recordStream(t.storage().data_ptr(), current_);
         return t;
+    }
+    void uses(std::initializer_list<const at::Tensor*> given) const {
+        if (stream_ == current_) return;
+        for (const at::Tensor* t : given)
+            if (t->defined() && t->numel())
+                c10::cuda::CUDACachingAllocator::recordStream(t->storage().data_ptr(), stream_);
     }
     // Runs f(stream), a C entry, and raises PaxError for its status.
     template <typename F>
@@ -198,6 +205,7 @@ PyObject* glu(PyObject* const* a) {
     }
     const bool save = given(g) || a[4] == Py_True;
     const Call call(dev, a[8]);
+    call.uses({&X, &Wg, &Wu, &H, &G, &U});
     if (!given(out)) H = call.empty({M, F}, at::kHalf);
     if (save && !given(g)) {
         G = call.empty({M, F}, at::kHalf);
@@ -246,6 +254,7 @@ PyObject* glu_backward(PyObject* const* a) {
         d.lddwu = matrix(dWu = tensor(pu, "dWu"), "dWu", D, F, wt, dev);
     }
     const Call call(dev, a[16]);
+    call.uses({&dH, &X, &Wg, &Wu, &G, &U, &dX, &dWg, &dWu, &dG, &dU});
     if (need_x && !given(px)) dX = call.empty({M, D}, at::kHalf);
     if (need_w && !given(pg)) {
         dWg = call.empty({D, F}, wt);
@@ -274,6 +283,7 @@ PyObject* quantize_rows(PyObject* const* a) {
     if (given(a[1])) ldq = matrix(Q = tensor(a[1], "out"), "out", M, K, at::kChar, dev);
     if (given(a[2])) vector(scale = tensor(a[2], "scale"), "scale", M, at::kFloat, dev);
     const Call call(dev, a[3]);
+    call.uses({&X, &Q, &scale});
     if (!given(a[1])) Q = call.empty({M, K}, at::kChar);
     if (!given(a[2])) scale = call.empty({M}, at::kFloat);
     call.run("pax_quantize_rows", [&](cudaStream_t s) {
@@ -306,6 +316,7 @@ PyObject* gemm_i8(PyObject* const* a) {
         d.ldc = matrix(C, "out", M, N, ct, dev);
     }
     const Call call(dev, a[7]);
+    call.uses({&A, &B, &sa, &sb, &bias, &C});
     if (!given(a[5])) C = call.empty({M, N}, ct);
     d.A = A.data_ptr(), d.B = B.data_ptr(), d.C = C.data_ptr();
     d.a_scale = static_cast<const float*>(sa.data_ptr());

@@ -6,7 +6,9 @@ pax_gemm_i8_ex).
 
 Every call is asynchronous on the current stream of the tensors' device, or on
 ``stream``, whatever device is current.  A new output belongs to that stream:
-a caller that passes ``stream`` orders its own use of the output after it.
+a caller that passes ``stream`` orders its own use of the output after it, and
+that stream's work after what writes the inputs.  The inputs themselves may be
+freed right after the call.
 Outputs must not overlap inputs or each other, but for glu_backward's dG and dU.
 autograd records none of the calls: glu_backward is called by hand.
 """

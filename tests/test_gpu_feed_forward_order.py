@@ -93,3 +93,28 @@ def test_waits_count_from_the_end_of_the_kernel_before(cuda, before, after):
             assert torch.equal(got, want)
     finally:
         assert lib.pax_selftest_set_wait_limit(0) == 0
+
+
+@pytest.mark.parametrize("call", ["glu", "glu_backward", "quantize_rows", "gemm_i8"])
+def test_inputs_freed_after_a_call_on_another_stream_are_not_reused_under_it(gen, call):
+    """torch's allocator hands memory that the caller frees to the next tensor of the current stream at once, unless it knows
+    that another stream still reads it."""
+    M, D, F = 512, 256, 512
+    make = {"glu": lambda: [randn(gen, M, D), *weights(gen, D, F)], "glu_backward": lambda: [t.clone() for t in back_inputs(gen, M, D, F)],
+            "quantize_rows": lambda: [randn(gen, M, D)],
+            "gemm_i8": lambda: [codes(gen, M, D), codes(gen, F, D), torch.ones(M, device=gen.device), torch.ones(F, device=gen.device)]}[call]
+    getattr(pax_b200, call)(*make())
+    s = torch.cuda.Stream()
+    a = make()
+    torch.cuda.synchronize()
+    with torch.cuda.stream(s):
+        torch.cuda._sleep(200_000_000)  # about 0.1 s
+    out = getattr(pax_b200, call)(*a, stream=s)
+    sizes, was = [(t.numel(), t.dtype) for t in a], {t.data_ptr() for t in a}
+    del a
+    fresh = [torch.empty(n, device=gen.device, dtype=t) for n, t in sizes]
+    busy = not s.query()
+    again = was & {t.data_ptr() for t in fresh}
+    torch.cuda.synchronize()
+    del out
+    assert busy and not again
