@@ -159,6 +159,14 @@ private:
     c10::cuda::CUDAStream current_, stream_;
 };
 
+// Counts outputs as written, as torch's own writes do: autograd refuses
+// a backward pass through a saved tensor that was overwritten.  Tensors made in
+// inference mode have no count.
+void written(std::initializer_list<const at::Tensor*> outs) {
+    for (const at::Tensor* t : outs)
+        if (t->defined() && !t->is_inference()) t->unsafeGetTensorImpl()->bump_version();
+}
+
 // A given output as it is, or a new tensor.
 PyObject* wrap(PyObject* out, const at::Tensor& t) {
     if (given(out)) {
@@ -214,6 +222,7 @@ PyObject* glu(PyObject* const* a) {
     d.X = X.data_ptr(), d.Wg = Wg.data_ptr(), d.Wu = Wu.data_ptr(), d.H = H.data_ptr();
     if (save) d.G = G.data_ptr(), d.U = U.data_ptr();
     call.run("pax_glu_ex", [&](cudaStream_t s) { return pax_glu_ex(&d, s); });
+    written({&H, &G, &U});
     if (!save) return wrap(out, H);
     return tuple({wrap(out, H), wrap(g, G), wrap(u, U)});
 }
@@ -269,6 +278,7 @@ PyObject* glu_backward(PyObject* const* a) {
     d.dw_dtype = wt == at::kHalf ? PAX_DT_F16 : PAX_DT_F32;
     d.accumulate = accumulate;
     call.run("pax_glu_backward_ex", [&](cudaStream_t s) { return pax_glu_backward_ex(&d, s); });
+    written({&dX, &dWg, &dWu, &dG, &dU});
     return tuple({need_x ? wrap(px, dX) : none(), need_w ? wrap(pg, dWg) : none(), need_w ? wrap(pu, dWu) : none()});
 }
 
@@ -289,6 +299,7 @@ PyObject* quantize_rows(PyObject* const* a) {
     call.run("pax_quantize_rows", [&](cudaStream_t s) {
         return pax_quantize_rows(X.data_ptr(), ldx, Q.data_ptr(), ldq, static_cast<float*>(scale.data_ptr()), M, K, s);
     });
+    written({&Q, &scale});
     return tuple({wrap(a[1], Q), wrap(a[2], scale)});
 }
 
@@ -324,6 +335,7 @@ PyObject* gemm_i8(PyObject* const* a) {
     if (given(a[4])) d.bias = bias.data_ptr();
     d.c_dtype = ct == at::kHalf ? PAX_DT_F16 : PAX_DT_F32;
     call.run("pax_gemm_i8_ex", [&](cudaStream_t s) { return pax_gemm_i8_ex(&d, s); });
+    written({&C});
     return wrap(a[5], C);
 }
 

@@ -10,7 +10,8 @@ a caller that passes ``stream`` orders its own use of the output after it, and
 that stream's work after what writes the inputs.  The inputs themselves may be
 freed right after the call.
 Outputs must not overlap inputs or each other, but for glu_backward's dG and dU.
-autograd records none of the calls: glu_backward is called by hand.
+autograd records none of the calls, whatever their inputs require:
+glu_backward is called by hand.  It does see that a given output was written.
 """
 from __future__ import annotations
 

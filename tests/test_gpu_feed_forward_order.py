@@ -118,3 +118,32 @@ def test_inputs_freed_after_a_call_on_another_stream_are_not_reused_under_it(gen
     torch.cuda.synchronize()
     del out
     assert busy and not again
+
+
+def test_outputs_that_a_caller_gives_count_as_written(gen):
+    """autograd refuses a backward pass through a saved tensor that was overwritten: it goes by the tensor's version."""
+    M, D, F = 40, 64, 72
+    X, (Wg, Wu) = randn(gen, M, D), weights(gen, D, F)
+    new = lambda *s, dt=F16: torch.zeros(s, device=gen.device, dtype=dt)  # noqa: E731
+    H, G, U = new(M, F), new(M, F), new(M, F)
+    dX, dWg, dWu = new(M, D), new(D, F, dt=F32), new(D, F, dt=F32)
+    Q, s, C = new(M, D, dt=I8), new(M, dt=F32), new(M, F)
+    B, sb = codes(gen, F, D), torch.ones(F, device=gen.device)
+    saved = G.float().requires_grad_(True)
+    for given, call in (((H, G, U), lambda: pax_b200.glu(X, Wg, Wu, out=H, G=G, U=U)),
+                        ((G, U, dX, dWg, dWu), lambda: pax_b200.glu_backward(H, X, Wg, Wu, G, U, dG=G, dU=U, dX=dX, dWg=dWg, dWu=dWu, accumulate=True)),
+                        ((Q, s), lambda: pax_b200.quantize_rows(X, out=Q, scale=s)), ((C,), lambda: pax_b200.gemm_i8(Q, B, s, sb, out=C))):
+        was, inputs = [t._version for t in given], [t._version for t in (X, Wg, Wu, B, sb)]
+        call()
+        assert all(t._version > v for t, v in zip(given, was))
+        assert [t._version for t in (X, Wg, Wu, B, sb)] == inputs
+    y = (saved * G.float() * G.float()).sum()
+    y2 = (torch.nn.functional.silu(saved.half()) * G).sum()
+    pax_b200.glu(X, Wg, Wu, out=H, G=G, U=U)
+    with pytest.raises(RuntimeError, match="modified by an inplace"):
+        y2.backward()
+    y.backward()
+    with torch.inference_mode():
+        T = new(M, F)
+        pax_b200.glu(X, Wg, Wu, out=T)
+    assert torch.equal(pax_b200.glu(X, Wg, Wu, out=T), H)  # tensors without a version
