@@ -26,11 +26,16 @@ bool dim_ok(long long v) { return v >= 0 && v <= kMaxDim; }
 
 // A matrix operand of T: rows x cols with its leading dimension (0: cols).
 // False when it has elements but no base, a base that is not aligned to its
-// elements, or overlapping rows.
+// elements, or overlapping rows.  A single row has no pitch; it gets one that
+// any kernel takes, so that its length alone keeps no product off the
+// tensor-core kernels (one token of 1001 features beside padded weights).
 bool matrix_ok_sized(const void* base, size_t elem, long long rows, long long cols, long long* ld) {
     if (*ld == 0) *ld = cols;
     if (rows == 0 || cols == 0) return true;
-    return base != nullptr && reinterpret_cast<uintptr_t>(base) % elem == 0 && *ld >= cols && *ld < (1LL << 38);
+    if (base == nullptr || reinterpret_cast<uintptr_t>(base) % elem != 0 || *ld < cols || *ld >= (1LL << 38))
+        return false;
+    if (rows == 1) *ld = (cols + 15) / 16 * 16;
+    return true;
 }
 template <typename T>
 bool matrix_ok(const T* base, long long rows, long long cols, long long* ld) {
