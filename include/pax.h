@@ -307,7 +307,9 @@ typedef enum {
 /* H = act(X.Wg) * (X.Wu), both products, the activation and the product in
  * one kernel.  G and U, both or neither, receive the two products X.Wg and
  * X.Wu, which pax_glu_backward_ex takes.  Sums are fp32; H is rounded to fp16
- * once, from the unrounded products. */
+ * once, from the unrounded products.  A product beyond fp16 (65504) is kept as
+ * an infinity in G or U, also where H is finite; the gradients of its element
+ * are then infinite or NaN. */
 typedef struct {
     const void*      X;  /* fp16 [M][ldx]    tokens                        */
     const void*      Wg; /* fp16 [D][ldwg]   gate projection               */
@@ -329,8 +331,13 @@ pax_status_t pax_glu_ex(const pax_glu_desc_t* desc, cudaStream_t stream);
  *   dG = dH * U * act'(G),  dU = dH * act(G)          (fp16 [M][F])
  *   dX = dG.Wg^T + dU.Wu^T                            (fp16 [M][D])
  *   dWg = X^T.dG,  dWu = X^T.dU                       (dw_dtype [D][F])
- * dG and dU are written too (they feed the two matrix products, rounded to
- * fp16) and may be the buffers of G and U themselves.  dX may be NULL, dWg
+ * dG and dU are written too, rounded to fp16: they are the operands of the two
+ * matrix products, which puts dX and the weight gradients at about 3e-4 of the
+ * exact values in the 2-norm (2e-4 for one rounding of an exact result).  Their
+ * range is fp16's as well: an element beyond 65504 becomes an infinity, and
+ * infinities and NaNs follow in dX and the weight gradients; one of 2^-25 or
+ * less becomes zero.  A caller scales dH for both, as with any fp16 gradients.
+ * dG and dU may be the buffers of G and U themselves.  dX may be NULL, dWg
  * and dWu may both be NULL; what is NULL is not computed.  accumulate != 0
  * adds dWg and dWu to what their buffers hold (fp32 only), each element once.
  * Equal inputs give equal bits from call to call. */
@@ -521,6 +528,17 @@ pax_status_t pax_selftest_set_wait_limit(uint64_t ns);
  * planned (round-robin tiles), -1 on a bad argument or too small a buffer. */
 int pax_selftest_wide_plan(long long M, long long N, long long K, int units, unsigned int* items, int* unit_start,
                            int max_items);
+/* Test hook (new; no counterpart in the reference; host only, launches
+ * nothing): the work that the tiles of pax_glu_ex (which = 0) or of both
+ * gradients of pax_glu_backward_ex (which = 1) deal out to `units` CTA pairs
+ * where a problem of M tokens, widths D and F runs on them.  Each item is five
+ * ints: the pair, 0 or for a weight gradient 1, the 256-row block, the first
+ * column (a weight gradient's: Wg's columns rounded up to whole tiles, then
+ * Wu's) and the number of columns.  *width: 1 for tiles of 256 accumulator
+ * columns, 2 for 512.  Returns the number of items, -1 on a bad argument or
+ * too small a buffer. */
+int pax_selftest_feed_forward_items(int which, long long M, long long D, long long F, int units, int* width, int* items,
+                                    int max_items);
 
 /* Frees the device memory this library allocated on its own: the skinny
  * kernel's per-stream workspaces and the planned tile tables of the wide

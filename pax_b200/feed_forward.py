@@ -65,7 +65,7 @@ def glu(X: torch.Tensor, Wg: torch.Tensor, Wu: torch.Tensor, *, activation="silu
     X [M, D], Wg and Wu [D, F] are float16 with unit column stride; H is
     float16 [M, F].  activation is one of silu, gelu_tanh, gelu_erf.  With
     ``save`` (or given G and U) the products X @ Wg and X @ Wu are kept for
-    glu_backward, and (H, G, U) is returned instead of H.
+    glu_backward, in float16, and (H, G, U) is returned instead of H.
     w_const: Wg and Wu are not written by the kernel launched just before on
     this stream (weights); with at most 64 tokens the kernel may then start
     reading them before that kernel ends (as gemm's b_const).
@@ -86,6 +86,10 @@ def glu_backward(dH: torch.Tensor, X: torch.Tensor, Wg: torch.Tensor, Wu: torch.
     the given float32 dWg and dWu.  dG and dU take the gradients of the two
     products and may be G and U themselves, which saves 2 M F values of
     scratch; by default they are scratch of the call.
+
+    dG and dU are rounded to float16 between the two steps: beyond 65504 they
+    become infinities, which reach dX and the weight gradients, and at 2^-25 or
+    less zeros.  dH is scaled for that by the caller, as float16 gradients are.
     """
     if dW_dtype not in _DT:
         raise TypeError("weight gradients must be float32 or float16")

@@ -112,3 +112,60 @@ def test_glu_backward_keeps_the_gates_tails(gen, name, size, shape):
         tol = t + 2.0 ** -11 * (want.abs() + t) + 2.0 ** -25
         bad = ((got.double() - want).abs() > tol) & (want.abs() < 65000)
         assert not bad.any(), (what, int(bad.sum()), g[bad][0].item(), got[bad][0].item(), want[bad][0].item())
+
+
+# ------------------------------------------------------------------ beyond fp16
+@pytest.mark.parametrize("M,D,F", [(5, 64, 72), (40, 264, 136), (300, 136, 520), (50, 65, 77)])
+def test_what_is_not_finite_stays_in_its_token(gen, M, D, F):
+    """A NaN or an infinity in a token's dH, U or X reaches that token's dX, or none, and the weight gradients; other tokens keep
+    their bits."""
+    a = [randn(gen, M, F), randn(gen, M, D), randn(gen, D, F, scale=0.1), randn(gen, D, F, scale=0.1), randn(gen, M, F), randn(gen, M, F)]
+    clean = pax_b200.glu_backward(*a)
+    for i in (0, 5):
+        for v in (float("nan"), float("inf")):
+            b = [t.clone() for t in a]
+            b[i][2, 3] = v
+            dX, dWg, dWu = pax_b200.glu_backward(*b)
+            rest = [m for m in range(M) if m != 2]
+            assert torch.equal(dX[rest], clean[0][rest]) and not dX[2].isfinite().any()
+            cols = [f for f in range(F) if f != 3]
+            assert torch.equal(dWg[:, cols], clean[1][:, cols]) and not dWg[:, 3].isfinite().any()
+            assert torch.equal(dWu[:, cols], clean[2][:, cols]) and (i == 5 or not dWu[:, 3].isfinite().any())
+    b = [t.clone() for t in a]
+    b[1][2, 3] = float("nan")
+    dX, dWg, _ = pax_b200.glu_backward(*b)
+    rest = [d for d in range(D) if d != 3]
+    assert torch.equal(dX, clean[0]) and dWg[3].isnan().all() and torch.equal(dWg[rest], clean[1][rest])
+
+
+@pytest.mark.parametrize("M", [9, 200])
+def test_products_of_the_gradient_beyond_fp16(gen, M):
+    """dG and dU are fp16, as pax.h says: what exceeds its range becomes an infinity, what is at most 2^-25 zero."""
+    F, D = 136, 64
+    G, one = torch.full((M, F), 40.0, device=gen.device, dtype=F16), torch.ones(M, F, device=gen.device, dtype=F16)
+    X, W = ints(gen, 1, M, D), ints(gen, 1, D, F)
+    dG, dU = torch.empty_like(G), torch.empty_like(G)
+    call = lambda dH, U: pax_b200.glu_backward(dH, X, W, W.clone(), G, U, dG=dG, dU=dU)  # noqa: E731  silu(40) = 40, silu' = 1
+    dX, dWg, dWu = call(512 * one, 200 * one)
+    assert (dG == float("inf")).all() and (dU == 512 * 40).all()
+    assert not dX[W.float().abs().sum(1).gt(0).expand(M, D)].isfinite().any() and not dWg[X.float().abs().sum(0) > 0].isfinite().any()
+    assert torch.equal(dWu, (X.double().T @ dU.double()).half())
+    call(-512 * one, 200 * one)
+    assert (dG == float("-inf")).all()
+    tiny = 2.0 ** -13 * one
+    call(tiny, 2.0 ** -12 * one)  # dG = 2^-25, half of the smallest fp16: to even
+    assert (dG == 0).all() and (dU == 40 * 2.0 ** -13).all()
+    call(tiny, 1.5 * 2.0 ** -12 * one)
+    assert (dG == 2.0 ** -24).all()
+
+
+@pytest.mark.parametrize("M", [9, 200])
+def test_gate_products_beyond_fp16(gen, M):
+    """H comes from the unrounded products: finite where G is kept as an infinity."""
+    D, F = 64, 136
+    X = torch.full((M, D), 64.0, device=gen.device, dtype=F16)
+    Wg, Wu = torch.full((D, F), -32.0, device=gen.device, dtype=F16), torch.full((D, F), 2.0 ** -14, device=gen.device, dtype=F16)
+    Wg[:, ::2] = 32.0
+    H, G, U = pax_b200.glu(X, Wg, Wu, save=True)  # g = -+131072, u = 1/4
+    assert (G[:, ::2] == float("inf")).all() and (G[:, 1::2] == float("-inf")).all() and (U == 0.25).all()
+    assert (H[:, ::2] == 32768).all() and (H[:, 1::2] == 0).all()
