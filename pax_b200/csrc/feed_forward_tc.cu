@@ -54,28 +54,37 @@ int ff_grid(const FfParams& p, int tiles, int units) {
     return items < units ? items : units;
 }
 
-template <int ACT>
-pax_status_t launch_glu(const FfMaps& maps, FfParams& p, cudaStream_t stream) {
-    const int units = ff_units<FF_GLU, ACT, __half, 1>(current_device());
-    const int units2 = ff_units<FF_GLU, ACT, __half, 2>(current_device());
-    if (units <= 0 || units2 <= 0) return PAX_ERR_CUDA;
+// The tile width of the gated product, 1 or 2, and its tiles for that many
+// CTA pairs of each width; the grid in pairs.
+int plan_glu(FfParams& p, int units, int units2, int& grid) {
     p.tiles_n = up(p.N, 128);
     const int tiles = p.tiles_m * p.tiles_n, tiles2 = p.tiles_m * up(p.N, 256);
     if (rounds(tiles2, units2) * tile_cost(2, p.kbs) < plan_pieces(p, tiles, units, 2)) {
         p.tiles_n = up(p.N, 256);
         p.full = tiles2;
         p.pieces = 1;
-        return ff_launch<FF_GLU, ACT, __half, 2>(maps, p, tiles2 < units2 ? tiles2 : units2, stream);
+        grid = tiles2 < units2 ? tiles2 : units2;
+        return 2;
     }
-    return ff_launch<FF_GLU, ACT, __half, 1>(maps, p, ff_grid(p, tiles, units), stream);
+    grid = ff_grid(p, tiles, units);
+    return 1;
 }
 
-template <typename OutT, int W>
-pax_status_t launch_back_w(const FfMaps& maps, FfParams& p, cudaStream_t stream) {
-    const int most = ff_units<FF_BACK, 0, OutT, W>(current_device());
-    if (most <= 0) return PAX_ERR_CUDA;
-    p.tiles_n = up(p.D, 256 * W);
-    p.wt_n = up(p.F, 256 * W);
+template <int ACT>
+pax_status_t launch_glu(const FfMaps& maps, FfParams& p, cudaStream_t stream) {
+    const int units = ff_units<FF_GLU, ACT, __half, 1>(current_device());
+    const int units2 = ff_units<FF_GLU, ACT, __half, 2>(current_device());
+    if (units <= 0 || units2 <= 0) return PAX_ERR_CUDA;
+    int grid;
+    return plan_glu(p, units, units2, grid) == 2 ? ff_launch<FF_GLU, ACT, __half, 2>(maps, p, grid, stream)
+                                                 : ff_launch<FF_GLU, ACT, __half, 1>(maps, p, grid, stream);
+}
+
+// The gradients' tiles of width w and their schedule on at most `most` CTA
+// pairs; the grid in pairs.
+int plan_back(FfParams& p, int w, int most) {
+    p.tiles_n = up(p.D, 256 * w);
+    p.wt_n = up(p.F, 256 * w);
     p.nx = p.nx ? p.tiles_m * p.tiles_n : 0;
     p.nw = p.nw ? p.wt_m * 2 * p.wt_n : 0;
     const long long items = (long long)p.nx + p.nw;
@@ -83,6 +92,14 @@ pax_status_t launch_back_w(const FfMaps& maps, FfParams& p, cudaStream_t stream)
     p.x_rem = p.nx % units;
     p.w_extra = 0;
     if (p.x_rem > 0 && p.nw > 0) p.w_extra = (p.kbs + p.kbs_w / 2) / p.kbs_w;
+    return units;
+}
+
+template <typename OutT, int W>
+pax_status_t launch_back_w(const FfMaps& maps, FfParams& p, cudaStream_t stream) {
+    const int most = ff_units<FF_BACK, 0, OutT, W>(current_device());
+    if (most <= 0) return PAX_ERR_CUDA;
+    const int units = plan_back(p, W, most);
     return ff_launch<FF_BACK, 0, OutT, W>(maps, p, units, stream);
 }
 // The time of both gradients in one launch with tiles of width w.  The weight
@@ -98,12 +115,13 @@ double back_time(const FfParams& p, int w, int units) {
     return t + (w == 1 ? kLastEpilogue : 0);
 }
 
+int back_width(const FfParams& p, int units) { return back_time(p, 2, units) < back_time(p, 1, units) ? 2 : 1; }
+
 template <typename OutT>
 pax_status_t launch_back(const FfMaps& maps, FfParams& p, cudaStream_t stream) {
     const int units = ff_units<FF_BACK, 0, OutT, 1>(current_device());
     if (units <= 0) return PAX_ERR_CUDA;
-    return back_time(p, 2, units) < back_time(p, 1, units) ? launch_back_w<OutT, 2>(maps, p, stream)
-                                                           : launch_back_w<OutT, 1>(maps, p, stream);
+    return back_width(p, units) == 2 ? launch_back_w<OutT, 2>(maps, p, stream) : launch_back_w<OutT, 1>(maps, p, stream);
 }
 
 template <typename OutT>
@@ -139,6 +157,14 @@ double glu_tc_time(const GluProblem& q) {
     return wide < narrow ? wide : narrow;
 }
 
+static void glu_params(const GluProblem& q, FfParams& p) {
+    p.M = (int)q.M;
+    p.N = (int)q.F;
+    p.tiles_m = up(q.M, 256);
+    p.kbs = up(q.D, 64);
+    p.group_m = kGroupM;
+}
+
 pax_status_t glu_tc(const GluProblem& q, cudaStream_t stream) {
     FfMaps maps;
     FfParams p = {};
@@ -152,11 +178,7 @@ pax_status_t glu_tc(const GluProblem& q, cudaStream_t stream) {
              matrix_map(&m[MG_U], q.U, kF16, 2, q.M, q.F, q.ldu, 64, 32);
     if (!ok) return PAX_ERR_CUDA;
     for (int i = q.G ? MG_U + 1 : MG_H + 1; i < 10; ++i) m[i] = m[MG_X];
-    p.M = (int)q.M;
-    p.N = (int)q.F;
-    p.tiles_m = up(q.M, 256);
-    p.kbs = up(q.D, 64);
-    p.group_m = kGroupM;
+    glu_params(q, p);
     p.save = q.G != nullptr;
     if (q.act == ACT_SILU) return launch_glu<ACT_SILU>(maps, p, stream);
     if (q.act == ACT_GELU_TANH) return launch_glu<ACT_GELU_TANH>(maps, p, stream);
@@ -222,6 +244,47 @@ pax_status_t glu_back_tc(const GluGradProblem& q, cudaStream_t stream) {
     return q.dw_f16 ? launch_back<__half>(maps, p, stream) : launch_back<float>(maps, p, stream);
 }
 
+// The items that the kernel's pairs run, as ff_item deals them out.
+template <int MODE, int W>
+static int list_items(const FfParams& p, int units, int* out, int max_items) {
+    int n = 0;
+    FfItem it;
+    for (int u = 0; u < units; ++u)
+        for (int idx = 0; ff_item<MODE, W>(p, u, units, idx, it); ++idx, ++n) {
+            if (n >= max_items) return -1;
+            int* o = out + 5 * n;
+            o[0] = u;
+            o[1] = it.kind;
+            o[2] = it.mb;
+            o[3] = MODE == FF_BACK ? it.nb * 256 * W : it.col;
+            o[4] = (MODE == FF_GLU ? it.w / 2 : it.w) * W;
+        }
+    return n;
+}
+
+int feed_forward_items(int which, long long M, long long D, long long F, int units, int* width, int* items,
+                       int max_items) {
+    FfParams p = {};
+    int w = 1, grid;
+    if (which == 0) {
+        GluProblem q = {};
+        q.M = M, q.D = D, q.F = F;
+        glu_params(q, p);
+        w = plan_glu(p, units, units, grid);
+    } else {
+        GluGradProblem q = {};
+        __half there;
+        q.M = M, q.D = D, q.F = F;
+        q.dX = &there, q.dWg = q.dWu = &there;
+        back_params(q, p);
+        w = back_width(p, units);
+        grid = plan_back(p, w, units);
+    }
+    *width = w;
+    if (which == 0) return w == 2 ? list_items<FF_GLU, 2>(p, grid, items, max_items) : list_items<FF_GLU, 1>(p, grid, items, max_items);
+    return w == 2 ? list_items<FF_BACK, 2>(p, grid, items, max_items) : list_items<FF_BACK, 1>(p, grid, items, max_items);
+}
+
 bool gemm_i8_tc_ok(const I8Problem& q) {
     return q.K > 0 && rows16(q.A, q.lda, 1) && rows16(q.B, q.ldb, 1) && tiles_ok(up(q.M, 256), up(q.N, 256));
 }
@@ -272,3 +335,11 @@ bool set_wait_limit_ff_tc(unsigned long long ns) {
 }
 
 }  // namespace pax
+
+extern "C" int pax_selftest_feed_forward_items(int which, long long M, long long D, long long F, int units, int* width,
+                                               int* items, int max_items) {
+    if ((which != 0 && which != 1) || M <= 0 || D <= 0 || F <= 0 || M > (1 << 24) || D > (1 << 24) || F > (1 << 24) ||
+        units < 1 || !width || !items || max_items < 0)
+        return -1;
+    return pax::feed_forward_items(which, M, D, F, units, width, items, max_items);
+}
