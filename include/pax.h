@@ -295,8 +295,8 @@ pax_status_t pax_ipc_close(void* device_ptr);
  * run at once and be captured into graphs.  Zero leading dimensions mean
  * contiguous.  Dimensions are below 2^31 - 1024.  Outputs must not overlap inputs or
  * one another, except where a field says so.  Bases and row pitches that are
- * multiples of 16 bytes run on the tcgen05 / TMA kernels; any other layout
- * runs on a slower kernel, to the same accuracy.
+ * multiples of 16 bytes run on the tcgen05 / TMA kernels (a single row has no
+ * pitch); any other layout runs on a slower kernel, to the same accuracy.
  * ------------------------------------------------------------------------- */
 typedef enum {
     PAX_ACT_SILU      = 0, /* x / (1 + exp(-x))                              */

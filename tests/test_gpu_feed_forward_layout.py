@@ -5,7 +5,7 @@ import pytest
 import torch
 
 import pax_b200
-from _feed_forward import close, gemm_i8, glu, quantize
+from _feed_forward import close, gemm_i8, glu, glu_grad, quantize
 from test_gpu_feed_forward import F16, codes, gen, padded, randn  # noqa: F401
 
 pytestmark = pytest.mark.gpu
@@ -64,3 +64,18 @@ def test_one_feature_and_one_weight_row(gen):
         close(t, glu(X, Wg, Wu, "silu")[what], what)
     dX, dWg, dWu = pax_b200.glu_backward(randn(gen, M, F), X, Wg, Wu, randn(gen, M, F), randn(gen, M, F))
     assert dX.shape == (M, 1) and dWg.shape == dWu.shape == (1, F) and dWg.isfinite().all()
+
+
+@pytest.mark.parametrize("M", [1, 70, 600])
+@pytest.mark.parametrize("F", [136, 137])
+def test_weight_gradients_of_a_single_feature(gen, M, F):
+    """Weight gradients of one row, from tokens in padded rows and as a column of their own; what lies around stays."""
+    X, Wg, Wu, G, U, dH = randn(gen, M, 1), randn(gen, 1, F), randn(gen, 1, F), randn(gen, M, F), randn(gen, M, F), randn(gen, M, F)
+    ref = glu_grad(dH, X, Wg, Wu, G, U, "silu", dw_f16=False)
+    for x in (X, padded(X, 7)):
+        buf = [torch.full((3, F + 7), 7.0, device=gen.device) for _ in range(2)]
+        got = pax_b200.glu_backward(dH, x, Wg, Wu, G, U, dWg=buf[0][1:2, :F], dWu=buf[1][1:2, :F])
+        for t, what in zip(got, ("dX", "dWg", "dWu")):
+            close(t, ref[what], what)
+        for b in buf:
+            assert (b[0] == 7).all() and (b[2] == 7).all() and (b[1, F:] == 7).all()

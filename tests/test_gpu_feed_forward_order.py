@@ -147,3 +147,27 @@ def test_outputs_that_a_caller_gives_count_as_written(gen):
         T = new(M, F)
         pax_b200.glu(X, Wg, Wu, out=T)
     assert torch.equal(pax_b200.glu(X, Wg, Wu, out=T), H)  # tensors without a version
+
+
+@pytest.mark.parametrize("M", [7, 300])
+def test_another_stream_inside_a_capture(gen, M):
+    """A capture that forks to a second stream and joins it: the inputs and outputs of calls there are recorded for it."""
+    D, F = 264, 520
+    X, (Wg, Wu) = randn(gen, M, D), weights(gen, D, F)
+    want = pax_b200.glu(X, Wg, Wu, save=True)
+    grads = pax_b200.glu_backward(want[0], X, Wg, Wu, want[1], want[2])
+    side, graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        side.wait_stream(torch.cuda.current_stream())
+        a = X.clone()
+        side.wait_stream(torch.cuda.current_stream())
+        H, G, U = pax_b200.glu(a, Wg, Wu, save=True, stream=side)
+        got = pax_b200.glu_backward(H, a, Wg, Wu, G, U, stream=side)
+        del a
+        torch.cuda.current_stream().wait_stream(side)
+    for _ in range(3):
+        graph.replay()
+    torch.cuda.synchronize()
+    for t, w in zip((H, G, U, *got), (*want, *grads)):
+        assert torch.equal(t, w)
